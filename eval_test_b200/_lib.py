@@ -77,11 +77,24 @@ def load() -> ctypes.CDLL:
     lib.nvfp4_grouped_gemm_noalloc.argtypes = [ctypes.POINTER(Group), i, f, vp]
     for q in (lib.nvfp4_quantize_f32, lib.nvfp4_quantize_f16, lib.nvfp4_quantize_bf16):
         q.argtypes = [vp, vp, vp, i, i, i, vp]
+    ll = ctypes.c_longlong
+    lib.nvfp4_moe_plan.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, vp]
+    lib.nvfp4_moe_route.argtypes = [vp, i, ll, vp, i, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.nvfp4_moe_route_backward.argtypes = [vp, vp, i, ll, vp, vp, i, i, i, i, vp, vp]
+    lib.nvfp4_moe_dispatch.argtypes = [vp, i, ll, vp, vp, i, i, i, i, vp, vp]
+    lib.nvfp4_moe_combine.argtypes = [vp, i, ll, vp, vp, i, i, i, vp, i, vp]
+    lib.nvfp4_moe_combine_backward.argtypes = [vp, i, ll, vp, i, ll, vp, vp, vp, i, i, i, i, vp, vp, vp]
+    lib.nvfp4_moe_dispatch_nvfp4.argtypes = [vp, i, ll, vp, vp, vp, i, i, i, i, vp, vp, vp]
+    lib.nvfp4_moe_gemm.argtypes = [vp] * 8 + [i, i, i, i, f, vp]
+    lib.nvfp4_moe_dual_gemm.argtypes = [vp] * 10 + [i, i, i, i, f, vp]
+    lib.nvfp4_moe_dual_gemm_nvfp4.argtypes = [vp] * 11 + [i, i, i, i, f, vp]
     lib.nvfp4_device_status.argtypes = [i, i]
     lib.nvfp4_wait_selftest.argtypes = [i, ctypes.POINTER(ctypes.c_double), vp]
     lib.nvfp4_strerror.argtypes = [i]
     lib.nvfp4_strerror.restype = ctypes.c_char_p
-    for name in ("nvfp4_gemv", "nvfp4_gemm", "nvfp4_dual_gemm", "nvfp4_dual_gemm_nvfp4", "nvfp4_gemm_allgather", "nvfp4_dual_gemm_allgather", "nvfp4_grouped_gemm", "nvfp4_grouped_gemm_noalloc", "nvfp4_quantize_f32", "nvfp4_quantize_f16", "nvfp4_quantize_bf16", "nvfp4_device_status",
+    for name in ("nvfp4_gemv", "nvfp4_gemm", "nvfp4_dual_gemm", "nvfp4_dual_gemm_nvfp4", "nvfp4_gemm_allgather", "nvfp4_dual_gemm_allgather", "nvfp4_grouped_gemm", "nvfp4_grouped_gemm_noalloc", "nvfp4_quantize_f32", "nvfp4_quantize_f16", "nvfp4_quantize_bf16", "nvfp4_moe_plan", "nvfp4_moe_route", "nvfp4_moe_route_backward",
+                 "nvfp4_moe_dispatch", "nvfp4_moe_combine", "nvfp4_moe_combine_backward", "nvfp4_moe_dispatch_nvfp4",
+                 "nvfp4_moe_gemm", "nvfp4_moe_dual_gemm", "nvfp4_moe_dual_gemm_nvfp4", "nvfp4_device_status",
                  "nvfp4_wait_selftest", "nvfp4_abi_version", "nvfp4_shutdown"):
         getattr(lib, name).restype = i
     _lib = lib

@@ -1,0 +1,293 @@
+"""A mixture-of-experts layer around the NVFP4 products, with the group sizes on the device.
+
+The grouped GEMM (eval/nvfp4_grouped_gemm/reference.py:137-201) takes its group sizes as a host list.  Here the router
+runs on the GPU and nothing is copied back: every call is asynchronous on the current stream and can be captured into
+a graph.  One layer:
+
+    r = moe.route(logits, top_k)                                     # weights, experts, plan
+    a, sfa = moe.dispatch_nvfp4(x, r.plan)                           # tokens sorted by expert, quantised
+    h, sfh = moe.expert_dual_gemm_nvfp4(a, sfa, b1, sfb1, b2, sfb2, r.plan)
+    y = moe.expert_gemm(h, sfh, b3, sfb3, r.plan)                    # fp16 rows, sorted by expert
+    out = moe.combine(y, r.plan, r.weights, dtype=x.dtype)
+
+T tokens choose k of E experts each.  Copy ``i = t * k + j`` is choice j of token t; the copies are sorted stably by
+expert into ``T * k`` rows.  A choice whose expert id lies outside [0, E) (-1, say) is not routed and has no row; the rows
+behind the last routed copy are zero in every sorted buffer made here.
+
+Expert weights are one batched operand, as ``quantize.quantize_operand`` makes it of ``[E, N, K]``: packed codes
+``[N, K/2, E]`` and the 6-D swizzled view of their scales.  The gradients of the 16- and 32-bit operations are functions
+of their own (``*_backward``); there are none of the NVFP4 products.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _args, _lib, formats as F
+
+MAX_EXPERTS, MAX_CHOICES = 1024, 32
+_KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+class Plan(NamedTuple):
+    """How the copies of a batch are sorted; int32 tensors on the batch's device (``nvfp4_moe_plan``).  The tensors of one
+    plan share one allocation."""
+    offsets: torch.Tensor   # [E + 1] first row of each expert; offsets[E] rows are in use
+    tiles: torch.Tensor     # [E + 1] first 128-row tile of each expert
+    rows: torch.Tensor      # [T, k] row of a copy, -1: not routed
+    slots: torch.Tensor     # [T, k] row counted with every expert padded to whole tiles, -1: not routed
+    source: torch.Tensor    # [T * k] copy of a row, -1 behind the last
+
+    @property
+    def num_experts(self) -> int:
+        return self.offsets.shape[0] - 1
+
+    @property
+    def most_tiles(self) -> int:
+        """128-row tiles that this many copies can fill at most, whatever their experts."""
+        copies, experts = self.source.shape[0], self.num_experts
+        active = min(copies, experts)
+        return active + (copies - active) // 128
+
+
+class Routing(NamedTuple):
+    weights: torch.Tensor   # [T, k] float32
+    experts: torch.Tensor   # [T, k] int32, largest weight first; -1: fewer than k candidates
+    plan: Plan
+
+
+def _matrix(t: torch.Tensor, name: str, rows: int | None = None, cols: int | None = None) -> int:
+    """Checks ``[rows, cols]`` of a floating type whose rows are contiguous; returns the pitch in elements."""
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _KINDS):
+        raise ValueError(f"{name}: expected a CUDA float32 / float16 / bfloat16 matrix")
+    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise ValueError(f"{name}: expected shape {(rows, cols)}, got {tuple(t.shape)}")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name}: the rows have to be contiguous, got strides {t.stride()}")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _choices(t: torch.Tensor, name: str, dtype: torch.dtype, shape=None) -> None:
+    if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype == dtype and t.is_contiguous()):
+        raise ValueError(f"{name}: expected a contiguous CUDA {dtype} tensor [T, k]")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _same_device(device: torch.device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"all tensors have to be on one device, got {t.device} beside {device}")
+
+
+def _call(entry: str, device: torch.device, *args) -> None:
+    """An entry point on the tensors' device and torch's current stream there."""
+    fn, index = getattr(_lib.load(), entry), device.index
+    if torch.cuda.current_device() == index:
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if code:
+        _lib.check(code, entry)
+
+
+def _new_plan(T: int, k: int, E: int, device) -> Plan:
+    n = T * k
+    make = torch.empty if n else torch.zeros             # (no tokens: no launch, every expert starts at row 0)
+    offsets, tiles, rows, slots, source = make(2 * (E + 1) + 3 * n, dtype=torch.int32, device=device).split(
+        [E + 1, E + 1, n, n, n])
+    return Plan(offsets, tiles, rows.view(T, k), slots.view(T, k), source)
+
+
+def plan(experts: torch.Tensor, num_experts: int) -> Plan:
+    """Sorts the choices ``experts`` [T, k] (int32) stably by expert.  Ids outside [0, num_experts) are not routed; an expert
+    may stand in a token more than once."""
+    _choices(experts, "experts", torch.int32)
+    if not 1 <= num_experts <= MAX_EXPERTS:
+        raise ValueError(f"num_experts: expected 1 to {MAX_EXPERTS}, got {num_experts}")
+    T, k = experts.shape
+    p = _new_plan(T, k, num_experts, experts.device)
+    if T * k:
+        _call("nvfp4_moe_plan", experts.device, experts.data_ptr(), T, num_experts, k, *(t.data_ptr() for t in p))
+    return p
+
+
+def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torch.Tensor | None = None) -> Routing:
+    """The ``top_k`` largest of each row of ``logits`` [T, E], ties to the lowest index, with their softmax weights over
+    the chosen entries (``renormalize``) or over all, and the plan of that choice.
+
+    NaN and -inf entries, and the rows of tokens whose ``mask`` [T] (bool) is false, are never chosen and take no part in
+    the sum; where fewer than ``top_k`` candidates are left the expert is -1 and the weight 0.  Several +inf entries share
+    the whole weight."""
+    ld = _matrix(logits, "logits")
+    T, E = logits.shape
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"logits: expected 1 to {MAX_EXPERTS} experts, got {E}")
+    if not 1 <= top_k <= min(E, MAX_CHOICES):
+        raise ValueError(f"top_k: expected 1 to {min(E, MAX_CHOICES)}, got {top_k}")
+    device = logits.device
+    if mask is not None:
+        if mask.dtype != torch.bool or mask.shape != (T,) or not mask.is_contiguous():
+            raise ValueError(f"mask: expected a contiguous bool tensor of shape {(T,)}")
+        _same_device(device, mask)
+    weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
+    experts = torch.empty((T, top_k), dtype=torch.int32, device=device)
+    p = _new_plan(T, top_k, E, device)
+    if T:
+        _call("nvfp4_moe_route", device, logits.data_ptr(), _KINDS[logits.dtype], ld, None if mask is None else mask.data_ptr(),
+              T, E, top_k, int(renormalize), weights.data_ptr(), experts.data_ptr(), *(t.data_ptr() for t in p))
+    return Routing(weights, experts, p)
+
+
+def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor,
+                   renormalize: bool = True) -> torch.Tensor:
+    """Gradient of ``route``'s weights with respect to ``logits`` (same type and shape; contiguous), from what ``route``
+    took and returned.  Entries that took no part have gradient 0."""
+    ld = _matrix(logits, "logits")
+    T, E = logits.shape
+    _choices(experts, "experts", torch.int32)
+    k = experts.shape[1]
+    if not 1 <= E <= MAX_EXPERTS or not 1 <= k <= min(E, MAX_CHOICES):
+        raise ValueError(f"experts: expected 1 to {min(E, MAX_CHOICES)} choices of 1 to {MAX_EXPERTS} experts, got {k} of {E}")
+    _choices(experts, "experts", torch.int32, (T, k))
+    _choices(weights, "weights", torch.float32, (T, k))
+    _choices(grad_weights, "grad_weights", torch.float32, (T, k))
+    _same_device(logits.device, weights, experts, grad_weights)
+    out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+    if T:
+        _call("nvfp4_moe_route_backward", logits.device, grad_weights.data_ptr(), logits.data_ptr(), _KINDS[logits.dtype], ld,
+              weights.data_ptr(), experts.data_ptr(), T, E, k, int(renormalize), out.data_ptr())
+    return out
+
+
+def dispatch(x: torch.Tensor, plan: Plan) -> torch.Tensor:
+    """``x`` [T, H] -> [T * k, H] of the same type: every token's row at the rows of its copies."""
+    T, k = plan.rows.shape
+    ld = _matrix(x, "x", T)
+    H = x.shape[1]
+    _same_device(x.device, plan.rows)
+    out = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
+    if out.numel():
+        _call("nvfp4_moe_dispatch", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan.rows.data_ptr(), plan.offsets.data_ptr(), T,
+              plan.num_experts, k, H, out.data_ptr())
+    return out
+
+
+def dispatch_backward(grad_rows: torch.Tensor, plan: Plan) -> torch.Tensor:
+    """Gradient of ``dispatch``: ``grad_rows`` [T * k, H] -> [T, H], the sum over each token's copies in fp32."""
+    return combine(grad_rows, plan)
+
+
+def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
+    """``y`` [T * k, H], rows sorted by expert -> [T, H]: the sum of each token's rows times ``weights`` [T, k] (float32; none:
+    the plain sum), in fp32, rounded once to ``dtype`` (default: that of ``y``).  Choices that are not routed add nothing."""
+    T, k = plan.rows.shape
+    ld = _matrix(y, "y", T * k)
+    H = y.shape[1]
+    dtype = y.dtype if dtype is None else dtype
+    if dtype not in _KINDS:
+        raise ValueError(f"dtype: expected float32, float16 or bfloat16, got {dtype}")
+    if weights is not None:
+        _choices(weights, "weights", torch.float32, (T, k))
+    _same_device(y.device, plan.rows, weights)
+    make = torch.empty if k else torch.zeros
+    out = make((T, H), dtype=dtype, device=y.device)
+    if out.numel() and k:
+        _call("nvfp4_moe_combine", y.device, y.data_ptr(), _KINDS[y.dtype], ld, None if weights is None else weights.data_ptr(),
+              plan.rows.data_ptr(), T, k, H, out.data_ptr(), _KINDS[dtype])
+    return out
+
+
+def combine_backward(grad_out: torch.Tensor, y: torch.Tensor, plan: Plan, weights: torch.Tensor):
+    """Gradients of ``combine`` with weights: ``grad_out`` [T, H] -> (that of ``y``, same type, rows that belong to no copy 0;
+    that of ``weights`` [T, k], 0 where a choice is not routed)."""
+    T, k = plan.rows.shape
+    ldo, ld = _matrix(grad_out, "grad_out", T), _matrix(y, "y", T * k, grad_out.shape[1])
+    H = y.shape[1]
+    _choices(weights, "weights", torch.float32, (T, k))
+    _same_device(y.device, grad_out, plan.rows, weights)
+    dy = torch.empty((T * k, H), dtype=y.dtype, device=y.device)
+    dw = (torch.empty if H else torch.zeros)((T, k), dtype=torch.float32, device=y.device)
+    if dy.numel():
+        _call("nvfp4_moe_combine_backward", y.device, grad_out.data_ptr(), _KINDS[grad_out.dtype], ldo, y.data_ptr(), _KINDS[y.dtype],
+              ld, weights.data_ptr(), plan.rows.data_ptr(), plan.offsets.data_ptr(), T, plan.num_experts, k, H, dy.data_ptr(),
+              dw.data_ptr())
+    return dy, dw
+
+
+def dispatch_nvfp4(x: torch.Tensor, plan: Plan):
+    """``dispatch`` with the rows quantised as ``quantize.quantize_operand`` does: ``x`` [T, K] -> (operand
+    ``[T * k, K/2, 1]`` float4_e2m1fn_x2, 6-D swizzled scales of the experts' 128-row tiles, ``plan.most_tiles`` of them).
+    Scale bytes of rows that do not exist are not written.  K is a multiple of 64."""
+    T, k = plan.rows.shape
+    ld = _matrix(x, "x", T)
+    K = x.shape[1]
+    if K % 64 or not K:
+        raise ValueError(f"x: the width has to be a multiple of 64, got {K}")
+    _same_device(x.device, plan.rows)
+    packed = torch.empty((1, T * k, K // 2), dtype=torch.uint8, device=x.device)
+    rows = plan.most_tiles * 128
+    scales = torch.empty(F.sf_buffer_bytes(rows, K), dtype=torch.uint8, device=x.device)
+    if T * k:
+        _call("nvfp4_moe_dispatch_nvfp4", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan.rows.data_ptr(), plan.slots.data_ptr(),
+              plan.offsets.data_ptr(), T, plan.num_experts, k, K, packed.data_ptr(), scales.data_ptr())
+    return F.batch_last(packed).view(torch.float4_e2m1fn_x2), F.permuted_view(scales, rows, K, 1)
+
+
+def _products(a, sfa, weights, plan: Plan, alpha):
+    """Checks the operands of an expert product -> (pointers in the C order, alphas pointer, alpha, R, E, N, K, device)."""
+    R, E = plan.source.shape[0], plan.num_experts
+    device = a.device
+    if a.dim() != 3 or not a.is_cuda:
+        raise ValueError("a: expected the CUDA operand [T * k, K/2, 1] that dispatch_nvfp4 returns")
+    K, N = 2 * a.shape[1], weights[0].shape[0]
+    if K % 256 or not K:
+        raise ValueError(f"a: K has to be a multiple of 256, got {K}")
+    if N % 128 or not N:
+        raise ValueError(f"b: N has to be a multiple of 128, got {N}")
+    ptrs = [_args.operand_ptr(a, R, K // 2, 1, "a"), _args.scales_ptr(sfa, plan.most_tiles * 128, K, 1, "sfa")]
+    for i in range(0, len(weights), 2):
+        ptrs += [_args.operand_ptr(weights[i], N, K // 2, E, "b"), _args.scales_ptr(weights[i + 1], N, K, E, "sfb")]
+    _same_device(device, sfa, *weights, plan.rows)
+    alphas = None
+    if isinstance(alpha, torch.Tensor):
+        if alpha.dtype != torch.float32 or alpha.shape != (E,) or not alpha.is_contiguous():
+            raise ValueError(f"alpha: expected a number or a contiguous float32 tensor of shape {(E,)}")
+        _same_device(device, alpha)
+        alphas, alpha = alpha.data_ptr(), 1.0
+    return ptrs + [plan.offsets.data_ptr(), plan.tiles.data_ptr(), alphas], float(alpha), R, E, N, K, device
+
+
+def expert_gemm(a, sfa, b, sfb, plan: Plan, alpha=1.0) -> torch.Tensor:
+    """``y[r] = fp16(alpha_e * a[r] @ b_e^T)`` for every sorted row r of expert e -> fp16 [T * k, N].  ``a``, ``sfa`` as
+    ``dispatch_nvfp4`` or ``expert_dual_gemm_nvfp4`` returns them, ``b`` [N, K/2, E] with its 6-D scales; ``alpha`` a number
+    or a float32 tensor [E], the experts' global scales.  N is a multiple of 128, K of 256."""
+    ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b, sfb), plan, alpha)
+    c = torch.empty((R, N), dtype=torch.float16, device=device)
+    if R:
+        _call("nvfp4_moe_gemm", device, *ptrs, c.data_ptr(), R, E, N, K, alpha)
+    return c
+
+
+def expert_dual_gemm(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0) -> torch.Tensor:
+    """``fp16(silu(alpha_e * a[r] @ b1_e^T) * (alpha_e * a[r] @ b2_e^T))`` -> fp16 [T * k, N]; arguments as for
+    ``expert_gemm``."""
+    ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
+    c = torch.empty((R, N), dtype=torch.float16, device=device)
+    if R:
+        _call("nvfp4_moe_dual_gemm", device, *ptrs, c.data_ptr(), R, E, N, K, alpha)
+    return c
+
+
+def expert_dual_gemm_nvfp4(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0):
+    """``expert_dual_gemm`` with its rows quantised to NVFP4, bit for bit what quantising the fp16 rows gives -> (operand
+    ``[T * k, N/2, 1]``, 6-D scales): ``a`` and ``sfa`` of the next product of the same plan."""
+    ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
+    packed = torch.empty((1, R, N // 2), dtype=torch.uint8, device=device)
+    rows = plan.most_tiles * 128
+    scales = torch.empty(F.sf_buffer_bytes(rows, N), dtype=torch.uint8, device=device)
+    if R:
+        _call("nvfp4_moe_dual_gemm_nvfp4", device, *ptrs, packed.data_ptr(), scales.data_ptr(), R, E, N, K, alpha)
+    return F.batch_last(packed).view(torch.float4_e2m1fn_x2), F.permuted_view(scales, rows, N, 1)

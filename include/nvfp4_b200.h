@@ -133,6 +133,74 @@ int nvfp4_quantize_f32(const void* x, void* packed, void* sf_sw, int rows, int K
 int nvfp4_quantize_f16(const void* x, void* packed, void* sf_sw, int rows, int K, int L, void* stream);
 int nvfp4_quantize_bf16(const void* x, void* packed, void* sf_sw, int rows, int K, int L, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Mixture-of-experts layer around the products: router, tokens sorted by expert and back, the experts' products.
+ * T tokens choose k of E experts (E <= 1024, k <= 32 in the router); copy i = t*k + j is choice j of token t.  The copies
+ * are sorted stably by expert into R = T*k rows.  The group sizes stay on the device, so a whole layer can be captured
+ * into a graph (eval/nvfp4_grouped_gemm/reference.py:137-201 takes them as a host list).  An expert id outside [0, E)
+ * means "not routed": the copy has no row.  No entry point keeps a workspace: what it needs is an argument.
+ * Element types of activations: */
+enum { NVFP4_F32 = 0, NVFP4_F16 = 1, NVFP4_BF16 = 2 };
+
+/* The plan of a batch, from the choices experts [T][k] (int32):
+ *   offsets [E+1]  first row of each expert; offsets[E] rows are in use
+ *   tiles   [E+1]  first 128-row tile of each expert (the sum of ceil(rows/128) of the experts before it)
+ *   rows    [T][k] row of a copy, -1: none
+ *   slots   [T][k] 128 * tile + row in the tile: where the scales of the copy's row are, -1: none
+ *   source  [T*k]  copy of a row, -1 behind the last one
+ * all int32.  T, E, k > 0. */
+int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* rows, void* slots,
+                   void* source, void* stream);
+
+/* Router: weights [T][k] (fp32) and experts [T][k] (int32) of the k largest of each row of logits [T][E] (element type
+ * `kind`, rows `ld` elements apart), largest first, ties to the lowest index, and the plan of that choice.
+ * weight = exp(l - max) / sum over the chosen entries (renormalize != 0) or over all.  NaN and -inf entries and rows
+ * whose byte in mask [T] (may be NULL) is 0 are never chosen and take no part in the sum; fewer than k candidates leave
+ * experts -1 with weight 0.  k <= E. */
+int nvfp4_moe_route(const void* logits, int kind, long long ld, const void* mask, int T, int E, int k, int renormalize,
+                    void* weights, void* experts, void* offsets, void* tiles, void* rows, void* slots, void* source,
+                    void* stream);
+/* Its gradient: dlogits [T][E] (element type `kind`, contiguous) from dweights [T][k] (fp32), with the weights and
+ * experts that the router returned; 0 for entries that took no part. */
+int nvfp4_moe_route_backward(const void* dweights, const void* logits, int kind, long long ld, const void* weights,
+                             const void* experts, int T, int E, int k, int renormalize, void* dlogits, void* stream);
+
+/* xs[rows[t][j]] = x[t] for x [T][H] (rows `ld` elements apart), xs [T*k][H]; rows behind the last copy become 0. */
+int nvfp4_moe_dispatch(const void* x, int kind, long long ld, const void* rows, const void* offsets, int T, int E, int k,
+                       int H, void* xs, void* stream);
+/* out[t] = sum_j weights[t][j] * y[rows[t][j]] (weights NULL: 1, which is the gradient of nvfp4_moe_dispatch), summed
+ * in fp32 in ascending j and rounded once to out_kind.  y [T*k][H] with rows `ld` elements apart, out [T][H]. */
+int nvfp4_moe_combine(const void* y, int kind, long long ld, const void* weights, const void* rows, int T, int k, int H,
+                      void* out, int out_kind, void* stream);
+/* The gradient of nvfp4_moe_combine: dy [T*k][H] (`kind`; rows behind the last copy become 0) and dweights [T][k]
+ * (fp32; 0 where a copy has no row) from dout [T][H] (out_kind, rows `ldo` elements apart). */
+int nvfp4_moe_combine_backward(const void* dout, int out_kind, long long ldo, const void* y, int kind, long long ld,
+                               const void* weights, const void* rows, const void* offsets, int T, int E, int k, int H,
+                               void* dy, void* dweights, void* stream);
+
+/* nvfp4_moe_dispatch with the rows quantised as nvfp4_quantize_* does: packed [T*k][K/2] (rows behind the last copy
+ * become 0) and sf_sw, the scale atoms [tiles][K/64][512] of every expert's own 128-row tiles (bytes of rows that do
+ * not exist are left as they are).  At most min(T*k, E) + (T*k - min(T*k, E)) / 128 tiles.  K % 64 == 0; x and its pitch
+ * 16-byte aligned. */
+int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, const void* rows, const void* slots, const void* offsets,
+                             int T, int E, int k, int K, void* packed, void* sf_sw, void* stream);
+
+/* The experts' products: c[r] = fp16(alpha * alphas[e] * (a*sfa)[r] @ (b*sfb)[e]^T) for every row r of expert e;
+ * a [R][K/2] and sfa_sw as nvfp4_moe_dispatch_nvfp4 leaves them (R = T*k), b [E][N][K/2] with swizzled scales as one
+ * batched operand of nvfp4_gemm, alphas [E] fp32 or NULL, c [R][N]; rows behind the last copy become 0.
+ * N % 128 == 0, K % 256 == 0; c 32-byte aligned, the operands 16-byte aligned. */
+int nvfp4_moe_gemm(const void* a, const void* sfa_sw, const void* b, const void* sfb_sw, const void* offsets,
+                   const void* tiles, const void* alphas, void* c, int R, int E, int N, int K, float alpha, void* stream);
+/* c[r] = fp16(silu(x) * y), x and y the products with b1[e] and b2[e], both times alpha * alphas[e]. */
+int nvfp4_moe_dual_gemm(const void* a, const void* sfa_sw, const void* b1, const void* sfb1_sw, const void* b2,
+                        const void* sfb2_sw, const void* offsets, const void* tiles, const void* alphas, void* c, int R,
+                        int E, int N, int K, float alpha, void* stream);
+/* The same with the result quantised, ready to be `a` of the next product of the same plan: c_packed [R][N/2], sfc_sw
+ * [tiles][N/64][512]; bit for bit nvfp4_quantize_f16 of the fp16 rows. */
+int nvfp4_moe_dual_gemm_nvfp4(const void* a, const void* sfa_sw, const void* b1, const void* sfb1_sw, const void* b2,
+                              const void* sfb2_sw, const void* offsets, const void* tiles, const void* alphas,
+                              void* c_packed, void* sfc_sw, int R, int E, int N, int K, float alpha, void* stream);
+
 /* Last device-side status code of device `dev` (0 = none); clear != 0 resets it.
  * Call after synchronising the stream.  No counterpart in the reference, whose kernels spin
  * without bound (eval/nvfp4_grouped_gemm/submission.py:91-104). */
