@@ -8,7 +8,7 @@ from . import formats as F
 
 
 def _strides_match(t: torch.Tensor, want: tuple[int, ...]) -> bool:
-    return all(s == w for s, w, n in zip(t.stride(), want, t.shape) if n > 1)
+    return t.stride() == want or all(s == w for s, w, n in zip(t.stride(), want, t.shape) if n > 1)
 
 
 def operand_ptr(t: torch.Tensor, rows: int, k2: int, L: int, name: str) -> int:

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "nvfp4_internal.h"
 #include "ptx_sm100.cuh"
 
@@ -24,15 +26,76 @@ template <> struct ElemOf<NVFP4_BF16> { using type = __nv_bfloat16; };
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T from_f32(float v);
-template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// Unsigned word of a size: what is moved without being looked at.
+template <int BYTES> struct Bits;
+template <> struct Bits<16> { using type = uint4; };
+template <> struct Bits<8> { using type = uint2; };
+template <> struct Bits<4> { using type = uint32_t; };
+template <> struct Bits<2> { using type = uint16_t; };
 
-// N consecutive elements, read or written as one access (N * sizeof(T) = 2 .. 32 bytes, aligned to its size, at most 16).
+// N consecutive elements (2, 4, 8, 16 or 32 bytes) kept as they lie in memory, two 16-bit elements to a register, until
+// they are looked at: as arrays of 16-bit values the compiler gave each element a register of its own, and the kernels
+// with eight vectors in flight fell to a quarter of the SM's threads.  Aligned to its size, at most 16 bytes.
 template <typename T, int N>
-struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Vec {
-    T v[N];
+struct Vec {
+    static constexpr int BYTES = N * (int)sizeof(T), WORDS = (BYTES + 3) / 4;
+    uint32_t w[WORDS];
+
+    __device__ __forceinline__ void load(const T* p) {
+        if constexpr (BYTES >= 16) {
+#pragma unroll
+            for (int i = 0; i < WORDS / 4; i++) {
+                const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+            }
+        } else if constexpr (BYTES == 8) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x; w[1] = v.y;
+        } else if constexpr (BYTES == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
+        } else {
+            w[0] = *reinterpret_cast<const uint16_t*>(p);
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        if constexpr (BYTES >= 16) {
+#pragma unroll
+            for (int i = 0; i < WORDS / 4; i++)
+                reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+        } else if constexpr (BYTES == 8) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+        } else if constexpr (BYTES == 4) {
+            *reinterpret_cast<uint32_t*>(p) = w[0];
+        } else {
+            *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+        }
+    }
+    __device__ __forceinline__ float get(int q) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[q]);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(q & 1 ? w[q / 2] & 0xffff0000u : w[q / 2] << 16);
+        else return __half2float(__ushort_as_half((unsigned short)(q & 1 ? w[q / 2] >> 16 : w[q / 2])));
+    }
+    // from fp32, one rounding to the nearest
+    __device__ __forceinline__ void set(const float (&f)[N]) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int q = 0; q < N; q++) w[q] = __float_as_uint(f[q]);
+        } else if constexpr (N == 1) {
+            if constexpr (std::is_same_v<T, __half>) w[0] = __half_as_ushort(__float2half_rn(f[0]));
+            else w[0] = __bfloat16_as_ushort(__float2bfloat16_rn(f[0]));
+        } else {
+#pragma unroll
+            for (int q = 0; q < N / 2; q++) {
+                if constexpr (std::is_same_v<T, __half>) {
+                    const __half2 h = __floats2half2_rn(f[2 * q], f[2 * q + 1]);
+                    w[q] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * q], f[2 * q + 1]);
+                    w[q] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+            }
+        }
+    }
 };
 
 inline int elem_bytes(int kind) { return kind == NVFP4_F32 ? 4 : 2; }

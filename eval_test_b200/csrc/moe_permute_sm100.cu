@@ -35,121 +35,178 @@ __device__ __forceinline__ void zero_tail(V* out, long long row, const PermuteAr
         out[i] = zero;
 }
 
-template <int BYTES> struct Bits;
-template <> struct Bits<16> { using type = uint4; };
-template <> struct Bits<8> { using type = uint2; };
-template <> struct Bits<4> { using type = uint32_t; };
-template <> struct Bits<2> { using type = uint16_t; };
+// What one warp does at a time: `U * 32` vectors of one token's row.  Lane j holds the row of the token's choice j (-1:
+// none) and its weight; both are fetched one piece ahead, so that their latency does not stand in front of the rows'.
+// (Fewer than 2^31 pieces: checked by the caller.)
+template <int U, bool WEIGHTED>
+struct Pieces {
+    const int* rows;               // [T][k]
+    const float* weights;          // [T][k]
+    unsigned k, row_vecs, segs, n, step, i;
+    unsigned t, c;                 // this warp's token and this lane's first vector of the piece
+    unsigned next_t, next_seg;
+    int row, next_row;
+    float w, next_w;
 
-// One thread per vector of a token's row: one load, k stores.
-template <int BYTES>
+    __device__ __forceinline__ Pieces(const PermuteArgs& p, const float* weights_, int row_vecs_)
+        : rows(p.rows), weights(weights_), k(p.k), row_vecs(row_vecs_), segs((row_vecs_ + 32 * U - 1) / (32 * U)) {
+        n = (unsigned)p.T * segs;
+        step = gridDim.x * (blockDim.x >> 5);
+        i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+        fetch(i);
+        locate();
+    }
+    __device__ __forceinline__ void fetch(unsigned at) {
+        const unsigned lane = threadIdx.x & 31;
+        next_t = at / segs;
+        next_seg = at - next_t * segs;
+        next_row = -1;
+        next_w = 0.f;
+        if (at < n && lane < k) {
+            const size_t copy = (size_t)next_t * k + lane;
+            next_row = __ldg(rows + copy);
+            if (WEIGHTED) next_w = __ldg(weights + copy);
+        }
+    }
+    __device__ __forceinline__ void locate() {
+        t = next_t;
+        c = next_seg * (32 * U) + (threadIdx.x & 31);
+        row = next_row;
+        w = next_row >= 0 ? next_w : 0.f;       // (a choice that is not routed may have any weight)
+        fetch(i + step);
+    }
+    __device__ __forceinline__ bool more() const { return i < n; }
+    __device__ __forceinline__ void next() { i += step; locate(); }
+};
+
+// One load of a token's vector, k stores.
+template <int BYTES, int U>
 __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* __restrict__ x, long long ld, void* __restrict__ xs,
                                                        int row_vecs, const PermuteArgs p) {
     using V = typename Bits<BYTES>::type;
-    const long long n = (long long)p.T * row_vecs, step = (long long)gridDim.x * blockDim.x;
     V* out = reinterpret_cast<V*>(xs);
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-        const long long t = i / row_vecs;
-        const int c = (int)(i - t * row_vecs);
-        const V v = __ldg(reinterpret_cast<const V*>(x + t * ld) + c);
-        const int* r = p.rows + t * p.k;
+    for (Pieces<U, false> w(p, nullptr, row_vecs); w.more(); w.next()) {
+        const V* src = reinterpret_cast<const V*>(x + w.t * ld);
+        V v[U];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (w.c + 32 * u < row_vecs) v[u] = __ldg(src + w.c + 32 * u);
         for (int j = 0; j < p.k; j++) {
-            const int row = __ldg(r + j);
-            if (row >= 0) out[(long long)row * row_vecs + c] = v;
+            const int row = __shfl_sync(0xffffffffu, w.row, j);
+            if (row < 0) continue;
+            V* dst = out + (long long)row * row_vecs + w.c;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (w.c + 32 * u < row_vecs) dst[32 * u] = v[u];
         }
     }
     zero_tail(out, row_vecs, p);
 }
 
-// One thread per vector of an output row: up to eight rows' loads in flight.
-template <typename TI, typename TO, int VN>
-__global__ void __launch_bounds__(256) combine_kernel(const TI* __restrict__ y, long long ld, const float* __restrict__ weights,
-                                                      TO* __restrict__ out, int row_vecs, const PermuteArgs p) {
-    const long long n = (long long)p.T * row_vecs, step = (long long)gridDim.x * blockDim.x;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-        const long long t = i / row_vecs;
-        const int c = (int)(i - t * row_vecs);
-        float acc[VN] = {};
-        for (int j0 = 0; j0 < p.k; j0 += 8) {
-            int row[8];
-            float w[8];
-            Vec<TI, VN> v[8];
+// KU rows' loads of U vectors each are in flight at a time.  `pitch`: bytes between rows of y.
+template <typename TI, typename TO, int VN, int KU, int U, bool WEIGHTED>
+__global__ void __launch_bounds__(256, U == 2 ? 3 : 4) combine_kernel(const TI* __restrict__ y, unsigned pitch, const float* __restrict__ weights,
+                                                         TO* __restrict__ out, int row_vecs, const PermuteArgs p) {
+    for (Pieces<U, WEIGHTED> w(p, weights, row_vecs); w.more(); w.next()) {
+        float acc[U][VN] = {};
+        const char* at = reinterpret_cast<const char*>(y + (size_t)w.c * VN);
+        for (int j0 = 0; j0 < p.k; j0 += KU) {
+            Vec<TI, VN> v[KU][U] = {};
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                row[j] = j0 + j < p.k ? __ldg(p.rows + t * p.k + j0 + j) : -1;
-                w[j] = (weights && row[j] >= 0) ? __ldg(weights + t * p.k + j0 + j) : 1.0f;
+            for (int j = 0; j < KU; j++) {
+                const int row = __shfl_sync(0xffffffffu, w.row, j0 + j);     // (-1 from the k-th lane on)
+                const TI* src = reinterpret_cast<const TI*>(at + (unsigned long long)(unsigned)row * pitch);
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (row >= 0 && w.c + 32 * u < row_vecs) v[j][u].load(src + 32 * u * VN);
             }
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (row[j] >= 0) v[j] = *reinterpret_cast<const Vec<TI, VN>*>(y + (long long)row[j] * ld + (long long)c * VN);
+            for (int j = 0; j < KU; j++) {
+                const float wj = WEIGHTED ? __shfl_sync(0xffffffffu, w.w, j0 + j) : 1.0f;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (row[j] >= 0) {
+                for (int u = 0; u < U; u++)
 #pragma unroll
-                    for (int q = 0; q < VN; q++) acc[q] = fmaf(w[j], to_f32(v[j].v[q]), acc[q]);
-                }
+                    for (int q = 0; q < VN; q++) acc[u][q] = fmaf(wj, v[j][u].get(q), acc[u][q]);
+            }
         }
-        Vec<TO, VN> o;
 #pragma unroll
-        for (int q = 0; q < VN; q++) o.v[q] = from_f32<TO>(acc[q]);
-        *reinterpret_cast<Vec<TO, VN>*>(out + t * p.H + (long long)c * VN) = o;
+        for (int u = 0; u < U; u++) {
+            if (w.c + 32 * u >= row_vecs) break;
+            Vec<TO, VN> o;
+            o.set(acc[u]);
+            o.store(out + (size_t)w.t * p.H + (size_t)(w.c + 32 * u) * VN);
+        }
     }
 }
 
-// GROUP threads per token (a warp for short rows, a block for long ones): a vector of dout[t] is read once for up to
-// eight of the token's rows; their dot products stay in registers and are summed over the group at the end, in an
-// order that depends on the sizes alone.
-template <typename TI, typename TO, int VN, int GROUP>
-__global__ void __launch_bounds__(256) combine_backward_kernel(const TO* __restrict__ dout, long long ldo, const TI* __restrict__ y,
-                                                               long long ld, const float* __restrict__ weights,
-                                                               TI* __restrict__ dy, float* __restrict__ dw, int row_vecs,
-                                                               const PermuteArgs p) {
-    __shared__ float part[8][8];
+// GROUP threads per token (a warp, or a block for long rows): a vector of dout[t] is read once for KU of the token's
+// rows; their dot products stay in registers and are summed over the group at the end, in an order that depends on the
+// sizes alone.  `pitch`: bytes between rows of y.
+template <typename TI, typename TO, int VN, int GROUP, int KU, int U>
+__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* __restrict__ dout, long long ldo, const TI* __restrict__ y,
+                                                                  unsigned pitch, const float* __restrict__ weights,
+                                                                  TI* __restrict__ dy, float* __restrict__ dw, int row_vecs,
+                                                                  const PermuteArgs p) {
+    __shared__ float part[8][KU];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int in_group = threadIdx.x % GROUP;
     constexpr int PER_BLOCK = 256 / GROUP;
+    const unsigned out_pitch = (unsigned)p.H * (unsigned)sizeof(TI);
     for (long long t = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / GROUP; t < p.T; t += (long long)gridDim.x * PER_BLOCK) {
         const TO* d = dout + t * ldo;
-        for (int j0 = 0; j0 < p.k; j0 += 8) {
-            int row[8];
-            float w[8], acc[8];
+        for (int j0 = 0; j0 < p.k; j0 += KU) {
+            int row[KU];
+            float w[KU], acc[KU];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < KU; j++) {
                 row[j] = j0 + j < p.k ? __ldg(p.rows + t * p.k + j0 + j) : -1;
                 w[j] = row[j] >= 0 ? __ldg(weights + t * p.k + j0 + j) : 0.f;
                 acc[j] = 0.f;
             }
-            for (int c = in_group; c < row_vecs; c += GROUP) {
-                const Vec<TO, VN> dv = *reinterpret_cast<const Vec<TO, VN>*>(d + (long long)c * VN);
-                Vec<TI, VN> v[8];
+            for (int c = in_group; c < row_vecs; c += GROUP * U) {
+                Vec<TO, VN> dv[U] = {};
+                Vec<TI, VN> v[KU][U] = {};
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (row[j] >= 0) v[j] = *reinterpret_cast<const Vec<TI, VN>*>(y + (long long)row[j] * ld + (long long)c * VN);
+                for (int u = 0; u < U; u++)
+                    if (c + GROUP * u < row_vecs) dv[u].load(d + (size_t)(c + GROUP * u) * VN);
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    if (row[j] >= 0) {
-                        Vec<TI, VN> o;
+                for (int j = 0; j < KU; j++) {
+                    const TI* src = reinterpret_cast<const TI*>(reinterpret_cast<const char*>(y) + (unsigned long long)(unsigned)row[j] * pitch) + (size_t)c * VN;
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+                        if (row[j] >= 0 && c + GROUP * u < row_vecs) v[j][u].load(src + GROUP * u * VN);
+                }
+#pragma unroll
+                for (int j = 0; j < KU; j++) {
+                    TI* dst = reinterpret_cast<TI*>(reinterpret_cast<char*>(dy) + (unsigned long long)(unsigned)row[j] * out_pitch) + (size_t)c * VN;
+#pragma unroll
+                    for (int u = 0; u < U; u++) {
+                        float f[VN];
 #pragma unroll
                         for (int q = 0; q < VN; q++) {
-                            const float g = to_f32(dv.v[q]);
-                            acc[j] = fmaf(g, to_f32(v[j].v[q]), acc[j]);
-                            o.v[q] = from_f32<TI>(w[j] * g);
+                            const float g = dv[u].get(q);
+                            acc[j] = fmaf(g, v[j][u].get(q), acc[j]);
+                            f[q] = w[j] * g;
                         }
-                        *reinterpret_cast<Vec<TI, VN>*>(dy + (long long)row[j] * p.H + (long long)c * VN) = o;
+                        Vec<TI, VN> o;
+                        o.set(f);
+                        if (row[j] >= 0 && c + GROUP * u < row_vecs) o.store(dst + GROUP * u * VN);
                     }
+                }
             }
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
+            for (int j = 0; j < KU; j++) {
+                if (row[j] < 0) acc[j] = 0.f;             // (dout may hold infinities: they met the zeros of no row)
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
             }
             if constexpr (GROUP > 32) {
                 if (lane == 0) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) part[warp][j] = acc[j];
+                    for (int j = 0; j < KU; j++) part[warp][j] = acc[j];
                 }
                 __syncthreads();
-                if (threadIdx.x < 8 && j0 + threadIdx.x < p.k) {
+                if (threadIdx.x < KU && j0 + threadIdx.x < p.k) {
                     float s = 0.f;
 #pragma unroll
                     for (int q = 0; q < 8; q++) s += part[q][threadIdx.x];
@@ -159,60 +216,64 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(const TO* __restr
             } else {
                 float s = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j++)
+                for (int j = 0; j < KU; j++)
                     if (lane == j) s = acc[j];
-                if (lane < 8 && j0 + lane < p.k) dw[t * p.k + j0 + lane] = s;
+                if (lane < KU && j0 + lane < p.k) dw[t * p.k + j0 + lane] = s;
             }
         }
     }
-    zero_tail(reinterpret_cast<Vec<TI, VN>*>(dy), row_vecs, p);
+    zero_tail(reinterpret_cast<typename Bits<VN * sizeof(TI)>::type*>(dy), row_vecs, p);
 }
 
-// One thread per 16-element block of a token: quantised once, its codes and scale byte stored for each of the token's
-// rows.  Four neighbouring lanes hold the four k-blocks of one 4-byte group of a scale atom (K % 64 == 0).  The scale
-// atoms follow the experts' 128-row tiles: slots[t][j] is the row with every expert padded to whole tiles.
+// One thread per 32 elements of a token: quantised once, their codes (16 bytes) and scale bytes stored for each of the
+// token's rows.  Two neighbouring lanes hold the four k-blocks of one 4-byte group of a scale atom (K % 64 == 0).  The
+// scale atoms follow the experts' 128-row tiles: slots[t][j] is the row with every expert padded to whole tiles.
 template <int KIND>
 __global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* __restrict__ x, long long ld, const int* __restrict__ slots,
                                                              uint8_t* __restrict__ codes, uint8_t* __restrict__ sf_sw,
                                                              const PermuteArgs p) {
     using T = typename ElemOf<KIND>::type;
-    const int kbs = p.H / 16;
+    const int units = p.H / 32;
     const int lane = threadIdx.x & 31;
-    const long long n = (long long)p.T * kbs, step = (long long)gridDim.x * blockDim.x;
+    const long long n = (long long)p.T * units, step = (long long)gridDim.x * blockDim.x;
     for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i - lane < n; i += step) {
         const bool in = i < n;
-        const long long t = in ? i / kbs : 0;
-        const int kb = in ? (int)(i - t * kbs) : 0;
-        float xs[16];
+        const long long t = in ? i / units : 0;
+        const int c = in ? (int)(i - t * units) : 0;
+        float xs[32];
         constexpr int VN = 16 / (int)sizeof(T);
-        const Vec<T, VN>* src = reinterpret_cast<const Vec<T, VN>*>(reinterpret_cast<const T*>(x) + t * ld + (long long)kb * 16);
+        const T* src = reinterpret_cast<const T*>(x) + t * ld + (long long)c * 32;
 #pragma unroll
-        for (int v = 0; v < 16 / VN; v++) {
-            const Vec<T, VN> a = src[v];
+        for (int v = 0; v < 32 / VN; v++) {
+            Vec<T, VN> a;
+            a.load(src + v * VN);
 #pragma unroll
-            for (int q = 0; q < VN; q++) xs[v * VN + q] = to_f32(a.v[q]);
+            for (int q = 0; q < VN; q++) xs[v * VN + q] = a.get(q);
         }
-        uint32_t w0, w1;
-        const uint32_t s = quantize_block16(xs, w0, w1);
-        // (n is a multiple of 4, so the four lanes of a group are in range together)
-        uint32_t word = s;
-        word |= __shfl_down_sync(0xffffffffu, s, 1) << 8;
-        word |= __shfl_down_sync(0xffffffffu, s, 2) << 16;
-        word |= __shfl_down_sync(0xffffffffu, s, 3) << 24;
+        uint4 w;
+        uint32_t s = quantize_block16(xs, w.x, w.y);
+        s |= quantize_block16(xs + 16, w.z, w.w) << 8;
+        // (n is even, so the two lanes of a group are in range together)
+        s |= __shfl_down_sync(0xffffffffu, s, 1) << 16;
         if (!in) continue;
+        const int* rows = p.rows + t * p.k;
+        uint8_t* dst = codes + (long long)c * 16;
         for (int j = 0; j < p.k; j++) {
-            const int row = __ldg(p.rows + t * p.k + j);
+            const int row = __ldg(rows + j);
             if (row < 0) continue;
-            *reinterpret_cast<uint2*>(codes + ((long long)row * kbs + kb) * 8) = make_uint2(w0, w1);
-            if ((lane & 3) == 0) {
+            *reinterpret_cast<uint4*>(dst + (long long)row * units * 16) = w;
+            if ((lane & 1) == 0) {
                 const int slot = __ldg(slots + t * p.k + j);
-                const long long atom = (long long)(slot >> 7) * (kbs / 4) + kb / 4;
-                *reinterpret_cast<uint32_t*>(sf_sw + atom * 512 + (slot & 31) * 16 + ((slot & 127) >> 5) * 4) = word;
+                const long long atom = (long long)(slot >> 7) * (units / 2) + c / 2;
+                *reinterpret_cast<uint32_t*>(sf_sw + atom * 512 + (slot & 31) * 16 + ((slot & 127) >> 5) * 4) = s;
             }
         }
     }
-    zero_tail(reinterpret_cast<uint2*>(codes), kbs, p);
+    zero_tail(reinterpret_cast<uint4*>(codes), units, p);
 }
+
+// Vectors per lane: one as long as that gives every SM a few warps, else U.
+bool spread(long long T, int row_vecs, int dev) { return T * ((row_vecs + 31) / 32) <= 16ll * sm_count(dev); }
 
 // Blocks of a grid-stride launch over n threads: at most eight resident blocks per SM.
 int grid_for(long long n, int dev) {
@@ -234,7 +295,7 @@ int launched() {
 
 int check_sizes(int T, int k, int H, long long ld) {
     if (T <= 0 || k <= 0 || H <= 0 || ld < 0) return NVFP4_ERR_SHAPE;
-    if ((long long)T * k >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
+    if (k > MOE_MAX_CHOICES || (long long)T * k >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
     return NVFP4_OK;
 }
 
@@ -272,16 +333,23 @@ extern "C" int nvfp4_moe_dispatch(const void* x, int kind, long long ld, const v
     if (vec < size) return NVFP4_ERR_ALIGN;
     const PermuteArgs p{(const int*)rows, (const int*)offsets + E, T, k, H};
     const int row_vecs = (int)(row_bytes / vec);
-    const int grid = grid_for((long long)T * row_vecs, dev);
     cudaStream_t st = (cudaStream_t)stream;
-    const uint8_t* src = (const uint8_t*)x;
+    auto go = [&](auto bytes, auto u) {
+        constexpr int B = decltype(bytes)::value, U = decltype(u)::value;
+        const long long warps = (long long)T * ((row_vecs + 32 * U - 1) / (32 * U));
+        if (warps >= (1ll << 31)) return (int)NVFP4_ERR_UNSUPPORTED;
+        dispatch_kernel<B, U><<<grid_for(32 * warps, dev), 256, 0, st>>>((const uint8_t*)x, ld * size, xs, row_vecs, p);
+        return launched();
+    };
+    auto go_bytes = [&](auto bytes) {
+        return spread(T, row_vecs, dev) ? go(bytes, std::integral_constant<int, 1>()) : go(bytes, std::integral_constant<int, 4>());
+    };
     switch (vec) {
-        case 16: dispatch_kernel<16><<<grid, 256, 0, st>>>(src, ld * size, xs, row_vecs, p); break;
-        case 8: dispatch_kernel<8><<<grid, 256, 0, st>>>(src, ld * size, xs, row_vecs, p); break;
-        case 4: dispatch_kernel<4><<<grid, 256, 0, st>>>(src, ld * size, xs, row_vecs, p); break;
-        default: dispatch_kernel<2><<<grid, 256, 0, st>>>(src, ld * size, xs, row_vecs, p); break;
+        case 16: return go_bytes(std::integral_constant<int, 16>());
+        case 8: return go_bytes(std::integral_constant<int, 8>());
+        case 4: return go_bytes(std::integral_constant<int, 4>());
+        default: return go_bytes(std::integral_constant<int, 2>());
     }
-    return launched();
 }
 
 extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const void* weights, const void* rows, int T, int k, int H,
@@ -293,6 +361,7 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;
     if ((uintptr_t)y % elem_bytes(kind) || (uintptr_t)out % elem_bytes(out_kind) || (uintptr_t)weights % 4) return NVFP4_ERR_ALIGN;
+    if (ld * elem_bytes(kind) >= (1ll << 32)) return NVFP4_ERR_UNSUPPORTED;      // (the kernel's row pitch is 32-bit bytes)
     const PermuteArgs p{(const int*)rows, nullptr, T, k, H};
     cudaStream_t st = (cudaStream_t)stream;
     return by_type(kind, [&](auto ti) {
@@ -304,12 +373,26 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
             constexpr unsigned long long O = VN * sizeof(TO) < 16 ? VN * sizeof(TO) : 16;
             const bool wide = H % VN == 0 && ld % VN == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)out % O == 0;
             const int row_vecs = wide ? H / VN : H;
-            const int grid = grid_for((long long)T * row_vecs, dev);
-            if (wide)
-                combine_kernel<TI, TO, VN><<<grid, 256, 0, st>>>((const TI*)y, ld, (const float*)weights, (TO*)out, row_vecs, p);
-            else
-                combine_kernel<TI, TO, 1><<<grid, 256, 0, st>>>((const TI*)y, ld, (const float*)weights, (TO*)out, row_vecs, p);
-            return launched();
+            auto go = [&](auto vn, auto ku, auto u) {
+                constexpr int N = decltype(vn)::value, KU = decltype(ku)::value, U = decltype(u)::value;
+                const long long warps = (long long)T * ((row_vecs + 32 * U - 1) / (32 * U));
+                if (warps >= (1ll << 31)) return (int)NVFP4_ERR_UNSUPPORTED;
+                const int grid = grid_for(32 * warps, dev);
+                const unsigned pitch = (unsigned)(ld * sizeof(TI));
+                if (weights)
+                    combine_kernel<TI, TO, N, KU, U, true><<<grid, 256, 0, st>>>((const TI*)y, pitch, (const float*)weights, (TO*)out, row_vecs, p);
+                else
+                    combine_kernel<TI, TO, N, KU, U, false><<<grid, 256, 0, st>>>((const TI*)y, pitch, nullptr, (TO*)out, row_vecs, p);
+                return launched();
+            };
+            using std::integral_constant;
+            auto go_width = [&](auto vn) {
+                if (spread(T, row_vecs, dev)) return go(vn, integral_constant<int, 8>(), integral_constant<int, 1>());
+                if (k <= 2) return go(vn, integral_constant<int, 2>(), integral_constant<int, 2>());
+                if (k <= 4) return go(vn, integral_constant<int, 4>(), integral_constant<int, 2>());
+                return go(vn, integral_constant<int, 8>(), integral_constant<int, 1>());
+            };
+            return wide ? go_width(integral_constant<int, VN>()) : go_width(integral_constant<int, 1>());
         });
     });
 }
@@ -327,6 +410,7 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
     if ((uintptr_t)y % elem_bytes(kind) || (uintptr_t)dy % elem_bytes(kind) || (uintptr_t)dout % elem_bytes(out_kind) ||
         (uintptr_t)weights % 4 || (uintptr_t)dweights % 4)
         return NVFP4_ERR_ALIGN;
+    if (ld * elem_bytes(kind) >= (1ll << 32) || (long long)H * elem_bytes(kind) >= (1ll << 32)) return NVFP4_ERR_UNSUPPORTED;
     const PermuteArgs p{(const int*)rows, (const int*)offsets + E, T, k, H};
     cudaStream_t st = (cudaStream_t)stream;
     return by_type(kind, [&](auto ti) {
@@ -338,19 +422,25 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
             const bool wide = H % VN == 0 && ld % VN == 0 && ldo % VN == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)dy % 16 == 0 &&
                               (uintptr_t)dout % O == 0;
             const int row_vecs = wide ? H / VN : H;
-            // a warp per token while its lanes take at most four vectors each
+            // a warp per token where its lanes take at most four vectors each
             const bool warp = row_vecs <= 128;
             const int grid = grid_for((long long)T * (warp ? 32 : 256), dev);
-            auto go = [&](auto vn, auto group) {
-                combine_backward_kernel<TI, TO, decltype(vn)::value, decltype(group)::value><<<grid, 256, 0, st>>>(
-                    (const TO*)dout, ldo, (const TI*)y, ld, (const float*)weights, (TI*)dy, (float*)dweights, row_vecs, p);
+            auto go = [&](auto vn, auto group, auto ku, auto u) {
+                combine_backward_kernel<TI, TO, decltype(vn)::value, decltype(group)::value, decltype(ku)::value, decltype(u)::value>
+                    <<<grid, 256, 0, st>>>((const TO*)dout, ldo, (const TI*)y, (unsigned)(ld * sizeof(TI)), (const float*)weights, (TI*)dy,
+                                           (float*)dweights, row_vecs, p);
+                return launched();
             };
             using std::integral_constant;
-            if (wide && warp) go(integral_constant<int, VN>(), integral_constant<int, 32>());
-            else if (wide) go(integral_constant<int, VN>(), integral_constant<int, 256>());
-            else if (warp) go(integral_constant<int, 1>(), integral_constant<int, 32>());
-            else go(integral_constant<int, 1>(), integral_constant<int, 256>());
-            return launched();
+            auto go_group = [&](auto vn, auto group) {
+                if (k <= 2) return go(vn, group, integral_constant<int, 2>(), integral_constant<int, 2>());
+                if (k <= 4) return go(vn, group, integral_constant<int, 4>(), integral_constant<int, 2>());
+                return go(vn, group, integral_constant<int, 8>(), integral_constant<int, 1>());
+            };
+            auto go_width = [&](auto vn) {
+                return warp ? go_group(vn, integral_constant<int, 32>()) : go_group(vn, integral_constant<int, 256>());
+            };
+            return wide ? go_width(integral_constant<int, VN>()) : go_width(integral_constant<int, 1>());
         });
     });
 }
@@ -363,11 +453,11 @@ extern "C" int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, c
     if (rc) return rc;
     if (E <= 0) return NVFP4_ERR_SHAPE;
     if (K % 64 != 0) return NVFP4_ERR_K_MULTIPLE;
-    if (((uintptr_t)x & 15) || ld * elem_bytes(kind) % 16 || ((uintptr_t)packed & 7) || ((uintptr_t)sf_sw & 3)) return NVFP4_ERR_ALIGN;
+    if (((uintptr_t)x & 15) || ld * elem_bytes(kind) % 16 || ((uintptr_t)packed & 15) || ((uintptr_t)sf_sw & 3)) return NVFP4_ERR_ALIGN;
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;
     const PermuteArgs p{(const int*)rows, (const int*)offsets + E, T, k, K};
-    const int grid = grid_for((long long)T * (K / 16), dev);
+    const int grid = grid_for((long long)T * (K / 32), dev);
     cudaStream_t st = (cudaStream_t)stream;
     switch (kind) {
         case NVFP4_F32: dispatch_quant_kernel<NVFP4_F32><<<grid, 256, 0, st>>>(x, ld, (const int*)slots, (uint8_t*)packed, (uint8_t*)sf_sw, p); break;

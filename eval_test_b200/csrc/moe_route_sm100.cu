@@ -12,6 +12,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "moe_common.cuh"
 
 namespace nvfp4 {
@@ -28,9 +30,15 @@ __device__ __forceinline__ float key_value(uint32_t k) {
 // exp(l - m) with the limit for m = +inf: entries equal to the maximum share the weight.
 __device__ __forceinline__ float exp_below(float l, float m) { return l == m ? 1.0f : expf(l - m); }
 
-__device__ __forceinline__ float warp_sum(float v) {
+// Over the G lanes of a token (every lane of the warp calls these).
+template <int G> __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <int G> __device__ __forceinline__ uint32_t group_max(uint32_t v) {
+#pragma unroll
+    for (int o = G / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
@@ -41,132 +49,205 @@ struct RouteArgs {
     float* weights;            // [T][k]
     int* experts;              // [T][k]
     int T, E, k, renormalize;
+    int wide;                  // rows start on 16-byte boundaries
 };
 
-// Keys of one token's row: lane holds the entries lane + 32 * i.
-template <int KIND, int NV>
-__device__ __forceinline__ void load_keys(const RouteArgs& a, int t, int lane, uint32_t (&key)[NV]) {
+// How a token's E entries lie in registers: G lanes with NV entries each, in pieces of VW neighbours (16 bytes), piece i
+// of lane l starting at entry (i * G + l) * VW.  A token takes a quarter of a warp up to 128 experts: the rounds of the
+// choice are bound by instruction issue, and the steps that reduce over lanes then serve four tokens at once (16384
+// tokens of 128 experts, k = 4: 9.4 us against 12.1 us with a warp per token and entries 32 apart).
+template <int KIND, int G_, int NV_> struct Layout {
     using T = typename ElemOf<KIND>::type;
-    const T* row = reinterpret_cast<const T*>(a.logits) + (long long)t * a.ld;
-    const bool live = !a.mask || a.mask[t] != 0;
+    static constexpr int G = G_, NV = NV_, VW = 16 / (int)sizeof(T), PER_WARP = 32 / G_;
+    // 16-bit logits: the order of a value takes at most 19 bits of its fp32 key, so its index fits below it and one
+    // maximum finds both
+    static constexpr bool PACKED = KIND != NVFP4_F32;
+    static constexpr int MINE = (MOE_MAX_CHOICES + G - 1) / G;     // choices that a lane keeps
+    static __device__ __forceinline__ int entry(int i, int in_group) { return ((i / VW) * G + in_group) * VW + i % VW; }
+    static __device__ __forceinline__ float value(uint32_t key) { return key_value(PACKED ? ((key & 0x80000000u) ? key & ~1023u : key | 1023u) : key); }
+};
+
+template <typename L>
+__device__ __forceinline__ void load_keys(const RouteArgs& a, int t, int in_group, uint32_t (&key)[L::NV]) {
+    using T = typename L::T;
+    const bool live = t < a.T && (!a.mask || a.mask[t] != 0);
+    const T* row = reinterpret_cast<const T*>(a.logits) + (long long)(live ? t : 0) * a.ld;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int e = i * 32 + lane;
-        float v = -INFINITY;
-        if (live && e < a.E) v = to_f32(row[e]);
-        key[i] = v > -INFINITY ? order_key(v) : 0u;      // (false for NaN)
+    for (int i = 0; i < L::NV; i += L::VW) {
+        const int e0 = L::entry(i, in_group);
+        Vec<T, L::VW> v;
+        const bool whole = a.wide && e0 + L::VW <= a.E;
+        if (live && whole) v.load(row + e0);
+#pragma unroll
+        for (int q = 0; q < L::VW; q++) {
+            float x = -INFINITY;
+            if (live && whole) x = v.get(q);
+            else if (live && e0 + q < a.E) x = to_f32(row[e0 + q]);
+            uint32_t k = x > -INFINITY ? order_key(x) : 0u;      // (false for NaN)
+            if (L::PACKED && k) k = (k & ~1023u) | (1023u - (uint32_t)(e0 + q));
+            key[i + q] = k;
+        }
     }
 }
 
-// One warp, one token.  k rounds of: the lane's best key, the warp's best key, the lowest index that has it.
-// 16384 tokens, 256 experts, k = 8: the rounds cost more than the 16 MB of logits.
-template <int KIND, int NV>
-__device__ __forceinline__ void route_token(const RouteArgs& a, int t, int lane) {
-    uint32_t key[NV];
-    load_keys<KIND, NV>(a, t, lane, key);
-    float total = 0.f, mine = 0.f, top = 0.f;
-    int chosen = -1;
-    uint32_t best = 0;
+// The tokens t of a warp's groups (t differs between groups, all lanes call it).  k rounds of: the lane's best key, the
+// group's best, the lowest index that has it; every lane of the group knows the choice, lane j % G keeps it.
+template <typename L>
+__device__ __forceinline__ void route_token(const RouteArgs& a, int t, int in_group) {
+    constexpr int G = L::G, NV = L::NV;
+    uint32_t key[NV], best = 0;
+    load_keys<L>(a, t, in_group, key);
 #pragma unroll
     for (int i = 0; i < NV; i++) best = max(best, key[i]);
+    float total = 0.f, top = 0.f, mine[L::MINE];
+    int chosen[L::MINE];
+#pragma unroll
+    for (int z = 0; z < L::MINE; z++) { mine[z] = 0.f; chosen[z] = -1; }
     for (int j = 0; j < a.k; j++) {
-        const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+        const uint32_t m = group_max<G>(best);                   // 0: no candidate is left
+        const float v = L::value(m);
         if (j == 0) {
-            top = key_value(m);
+            top = v;
             if (!a.renormalize) {
 #pragma unroll
-                for (int i = 0; i < NV; i++)
-                    if (key[i]) total += exp_below(key_value(key[i]), top);
-                total = warp_sum(total);
+                for (int i = 0; i < NV; i++) total += key[i] ? exp_below(L::value(key[i]), top) : 0.f;
+                total = group_sum<G>(total);
             }
         }
-        if (m == 0) break;                                // fewer than k entries are left
-        uint32_t at = 0xffffffffu;
-        if (best == m) {
-#pragma unroll
-            for (int i = NV - 1; i >= 0; i--)
-                if (key[i] == m) at = i * 32 + lane;
-        }
-        at = __reduce_min_sync(0xffffffffu, at);
-        if (lane == j) {
-            chosen = (int)at;
-            mine = exp_below(key_value(m), top);
-        }
-        if (lane == (int)(at & 31u)) {
+        uint32_t at;
+        if (L::PACKED) {
+            at = 1023u - (m & 1023u);
             best = 0;
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                if (i == (int)(at >> 5)) key[i] = 0;
+                key[i] = key[i] == m ? 0u : key[i];
+                best = max(best, key[i]);
+            }
+        } else {
+            // the lowest index that has the key, as the largest of their complements
+            uint32_t low = 0;
+#pragma unroll
+            for (int i = NV - 1; i >= 0; i--)
+                if (key[i] == m) low = 1024u - (uint32_t)L::entry(i, in_group);
+            at = 1024u - group_max<G>(low);
+            best = 0;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                if ((uint32_t)L::entry(i, in_group) == at) key[i] = 0u;
                 best = max(best, key[i]);
             }
         }
+        const float p = m ? exp_below(v, top) : 0.f;
+        if (a.renormalize) total += p;
+        if (in_group == j % G) {
+#pragma unroll
+            for (int z = 0; z < L::MINE; z++)
+                if (z == j / G) { mine[z] = p; chosen[z] = m ? (int)at : -1; }
+        }
     }
-    if (a.renormalize) total = warp_sum(mine);
-    if (lane < a.k) {
-        a.weights[(long long)t * a.k + lane] = chosen >= 0 ? mine / total : 0.f;
-        a.experts[(long long)t * a.k + lane] = chosen;
+    if (t < a.T) {
+#pragma unroll
+        for (int z = 0; z < L::MINE; z++) {
+            const int j = z * G + in_group;
+            if (j < a.k) {
+                a.weights[(long long)t * a.k + j] = chosen[z] >= 0 ? mine[z] / total : 0.f;
+                a.experts[(long long)t * a.k + j] = chosen[z];
+            }
+        }
     }
 }
 
-template <int KIND, int NV>
+template <typename L>
 __global__ void __launch_bounds__(256) route_kernel(const RouteArgs a) {
     const int lane = threadIdx.x & 31;
     const int warps = gridDim.x * (blockDim.x >> 5);
-    for (int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < a.T; t += warps) route_token<KIND, NV>(a, t, lane);
+    for (int t = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * L::PER_WARP; t < a.T; t += warps * L::PER_WARP)
+        route_token<L>(a, t + lane / L::G, lane % L::G);
 }
 
-// One warp, one token.  The chosen experts' terms are handed round by shuffles, so every entry is written once.
-template <int KIND, int NV>
+// G lanes, one token.  The chosen experts' terms are handed round by shuffles, so every entry is written once.
+template <typename L>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a, const float* __restrict__ dw, void* dlogits) {
-    using T = typename ElemOf<KIND>::type;
-    const int lane = threadIdx.x & 31;
+    using T = typename L::T;
+    constexpr int G = L::G, NV = L::NV;
+    const int lane = threadIdx.x & 31, in_group = lane % G;
     const int warps = gridDim.x * (blockDim.x >> 5);
-    for (int t = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < a.T; t += warps) {
-        int e = -1;
-        float w = 0.f, g = 0.f;
-        if (lane < a.k) {
-            e = a.experts[(long long)t * a.k + lane];
-            if ((unsigned)e < (unsigned)a.E) {
-                w = a.weights[(long long)t * a.k + lane];
-                g = dw[(long long)t * a.k + lane];
-            } else {
-                e = -1;
+    for (int t0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * L::PER_WARP; t0 < a.T; t0 += warps * L::PER_WARP) {
+        const int t = t0 + lane / G;
+        int e[L::MINE];
+        float w[L::MINE], g[L::MINE], dot = 0.f;
+        uint32_t any = 0;
+#pragma unroll
+        for (int z = 0; z < L::MINE; z++) {
+            const int j = z * G + in_group;
+            e[z] = -1; w[z] = g[z] = 0.f;
+            if (t < a.T && j < a.k) {
+                const int id = a.experts[(long long)t * a.k + j];
+                if ((unsigned)id < (unsigned)a.E) {
+                    e[z] = id;
+                    w[z] = a.weights[(long long)t * a.k + j];
+                    g[z] = dw[(long long)t * a.k + j];
+                    any = 1;
+                }
             }
+            dot += w[z] * g[z];
         }
-        const float dot = warp_sum(w * g);
-        const bool any = __any_sync(0xffffffffu, e >= 0);
+        dot = group_sum<G>(dot);
+        any = group_max<G>(any);
         float p[NV], d[NV];
         if (!a.renormalize) {
             uint32_t key[NV], best = 0;
-            load_keys<KIND, NV>(a, t, lane, key);
+            load_keys<L>(a, t, in_group, key);
 #pragma unroll
             for (int i = 0; i < NV; i++) best = max(best, key[i]);
-            const float top = key_value(__reduce_max_sync(0xffffffffu, best));
+            best = group_max<G>(best);
+            const float top = L::value(best);
             float total = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                p[i] = key[i] ? exp_below(key_value(key[i]), top) : 0.f;
+                p[i] = key[i] ? exp_below(L::value(key[i]), top) : 0.f;
                 total += p[i];
             }
-            total = warp_sum(total);
+            total = group_sum<G>(total);
+            // (a row without choices, a masked one say, has gradient 0)
+            const float scale = any ? 1.0f / total : 0.f;       // (one division for the row, an ulp more in its entries)
 #pragma unroll
-            for (int i = 0; i < NV; i++) p[i] = (any && total > 0.f) ? p[i] / total : 0.f;
+            for (int i = 0; i < NV; i++) p[i] *= scale;
         }
 #pragma unroll
         for (int i = 0; i < NV; i++) d[i] = a.renormalize ? 0.f : -dot;
-        const float own = a.renormalize ? w * (g - dot) : g;
-        for (int j = 0; j < a.k; j++) {
-            const int ej = __shfl_sync(0xffffffffu, e, j);
-            const float gj = __shfl_sync(0xffffffffu, own, j);
 #pragma unroll
-            for (int i = 0; i < NV; i++)
-                if (ej == i * 32 + lane) d[i] += gj;
+        for (int z = 0; z < L::MINE; z++) {
+            const float own = a.renormalize ? w[z] * (g[z] - dot) : g[z];
+            for (int j = z * G; j < a.k && j < (z + 1) * G; j++) {
+                const int ej = __shfl_sync(0xffffffffu, e[z], j - z * G, G);
+                const float gj = __shfl_sync(0xffffffffu, own, j - z * G, G);
+#pragma unroll
+                for (int i = 0; i < NV; i++)
+                    if (ej == L::entry(i, in_group)) d[i] += gj;
+            }
         }
+        if (t >= a.T) continue;
         T* row = reinterpret_cast<T*>(dlogits) + (long long)t * a.E;
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int idx = i * 32 + lane;
-            if (idx < a.E) row[idx] = from_f32<T>(a.renormalize ? d[i] : (p[i] > 0.f ? p[i] * d[i] : 0.f));
+        for (int i = 0; i < NV; i += L::VW) {
+            const int e0 = L::entry(i, in_group);
+            float f[L::VW];
+#pragma unroll
+            for (int q = 0; q < L::VW; q++) f[q] = a.renormalize ? d[i + q] : (p[i + q] > 0.f ? p[i + q] * d[i + q] : 0.f);
+            if (a.E % L::VW == 0) {                               // (dlogits is contiguous and 16-byte aligned)
+                Vec<T, L::VW> o;
+                o.set(f);
+                if (e0 < a.E) o.store(row + e0);
+            } else {
+#pragma unroll
+                for (int q = 0; q < L::VW; q++) {
+                    const float one[1] = {f[q]};
+                    Vec<T, 1> o;
+                    o.set(one);
+                    if (e0 + q < a.E) o.store(row + e0 + q);
+                }
+            }
         }
     }
 }
@@ -183,6 +264,7 @@ struct PlanArgs {
 };
 
 constexpr int PLAN_WARPS = 32;
+constexpr int PLAN_AHEAD = 8;      // rounds of 32 copies whose ids a warp has in flight
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
     uint32_t v;
@@ -195,12 +277,24 @@ __device__ __forceinline__ uint32_t cluster_size() {
     return r;
 }
 
+// Lanes whose key equals this lane's, by one vote per bit (match.any took 1900 cycles a round with a warp's 32 lanes at
+// 64 experts, the votes take 300).
+__device__ __forceinline__ uint32_t same_key(int key, int bits) {
+    uint32_t same = 0xffffffffu;
+    for (int b = 0; b < bits; b++) {
+        const bool one = (key >> b) & 1;
+        const uint32_t vote = __ballot_sync(0xffffffffu, one);
+        same &= one ? vote : ~vote;
+    }
+    return same;
+}
+
 // The whole sort is ONE cluster: every warp owns a contiguous run of tokens, counts its copies per expert, the counts
 // are summed over the warps of a CTA in its shared memory and over the CTAs through distributed shared memory, and a
 // second walk over the same copies hands out the rows in order.  No global scratch, no atomics, so the order is that
-// of the copies and a graph can replay it beside any other.  KIND >= 0: the warps choose their tokens' experts first
-// (few tokens: one launch for router and plan).
-template <int KIND, int NV>
+// of the copies and a graph can replay it beside any other.  L: the warps choose their tokens' experts first, in that
+// layout (few tokens: one launch for router and plan); void: the choices are given.
+template <typename L>
 __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs p, const RouteArgs a) {
     extern __shared__ uint32_t plan_smem[];
     uint32_t* hist = plan_smem;                         // [PLAN_WARPS][E]
@@ -217,18 +311,29 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     const int begin = t0 * p.k, end = t1 * p.k;         // (T * k < 2^31: checked by the caller)
 
     for (int i = threadIdx.x; i < PLAN_WARPS * p.E; i += blockDim.x) hist[i] = 0;
-    if constexpr (KIND >= 0) {
-        for (int t = t0; t < t1; t++) route_token<KIND, NV>(a, t, lane);
+    if constexpr (!std::is_void_v<L>) {
+        for (int t = t0; t < t1; t += L::PER_WARP) {
+            const int tg = t + lane / L::G;
+            route_token<L>(a, tg < t1 ? tg : a.T, lane % L::G);
+        }
     }
     __syncthreads();
     uint32_t* own = hist + warp * p.E;
-    for (int i0 = begin; i0 < end; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = i < end ? p.experts[i] : -1;
-        const bool ok = (unsigned)e < (unsigned)p.E;
-        const uint32_t same = __match_any_sync(0xffffffffu, ok ? e : -1);
-        if (ok && lane == __ffs(same) - 1) own[e] += __popc(same);
-        __syncwarp();
+    const int bits = 32 - __clz(p.E);                   // keys 0 .. E
+    // (eight loads in flight: one after the other they were most of the kernel's time)
+    for (int i0 = begin; i0 < end; i0 += 32 * PLAN_AHEAD) {
+        int ids[PLAN_AHEAD];
+#pragma unroll
+        for (int u = 0; u < PLAN_AHEAD; u++) ids[u] = i0 + 32 * u + lane < end ? p.experts[i0 + 32 * u + lane] : -1;
+#pragma unroll
+        for (int u = 0; u < PLAN_AHEAD; u++) {
+            if (i0 + 32 * u >= end) break;
+            const int e = ids[u];
+            const bool ok = (unsigned)e < (unsigned)p.E;
+            const uint32_t same = same_key(ok ? e : p.E, bits);
+            if (ok && lane == __ffs(same) - 1) own[e] += __popc(same);
+            __syncwarp();
+        }
     }
     __syncthreads();
     for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
@@ -274,27 +379,33 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     }
     // also: no CTA leaves while a peer may still read its counts
     cluster_sync_all();
-    for (int i0 = begin; i0 < end; i0 += 32) {
-        const int i = i0 + lane;
-        const int e = i < end ? p.experts[i] : -1;
-        const bool ok = (unsigned)e < (unsigned)p.E;
-        const uint32_t same = __match_any_sync(0xffffffffu, ok ? e : -1);
-        int row = -1, slot = -1;
-        if (ok) {
-            row = (int)(base[e] + own[e]) + __popc(same & ((1u << lane) - 1u));
-            slot = row + shift[e];
+    for (int i0 = begin; i0 < end; i0 += 32 * PLAN_AHEAD) {
+        int ids[PLAN_AHEAD];
+#pragma unroll
+        for (int u = 0; u < PLAN_AHEAD; u++) ids[u] = i0 + 32 * u + lane < end ? p.experts[i0 + 32 * u + lane] : -1;
+#pragma unroll
+        for (int u = 0; u < PLAN_AHEAD; u++) {
+            if (i0 + 32 * u >= end) break;
+            const int i = i0 + 32 * u + lane, e = ids[u];
+            const bool ok = (unsigned)e < (unsigned)p.E;
+            const uint32_t same = same_key(ok ? e : p.E, bits);
+            int row = -1, slot = -1;
+            if (ok) {
+                row = (int)(base[e] + own[e]) + __popc(same & ((1u << lane) - 1u));
+                slot = row + shift[e];
+            }
+            __syncwarp();
+            if (ok && lane == __ffs(same) - 1) own[e] += __popc(same);
+            __syncwarp();
+            if (i < end) { p.rows[i] = row; p.slots[i] = slot; }
+            if (ok) p.source[row] = i;
         }
-        __syncwarp();
-        if (ok && lane == __ffs(same) - 1) own[e] += __popc(same);
-        __syncwarp();
-        if (i < end) { p.rows[i] = row; p.slots[i] = slot; }
-        if (ok) p.source[row] = i;
     }
     const int n = p.T * p.k;
     for (long long i = (long long)live_rows + rank * blockDim.x + threadIdx.x; i < n; i += (long long)ctas * blockDim.x) p.source[i] = -1;
 }
 
-template <int KIND, int NV>
+template <typename L>
 int launch_plan(const PlanArgs& p, const RouteArgs& a, int ctas, cudaStream_t st) {
     static bool configured[64] = {};
     int dev = 0;
@@ -303,7 +414,7 @@ int launch_plan(const PlanArgs& p, const RouteArgs& a, int ctas, cudaStream_t st
     if (dev >= 64) return NVFP4_ERR_UNSUPPORTED;
     constexpr size_t most = (size_t)(PLAN_WARPS + 3) * MOE_MAX_EXPERTS * 4;
     if (!configured[dev]) {
-        e = cudaFuncSetAttribute(plan_kernel<KIND, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        e = cudaFuncSetAttribute(plan_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (e != cudaSuccess) return (int)e;
         configured[dev] = true;
     }
@@ -317,7 +428,7 @@ int launch_plan(const PlanArgs& p, const RouteArgs& a, int ctas, cudaStream_t st
     attr.val.clusterDim.x = ctas; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, plan_kernel<KIND, NV>, p, a);
+    e = cudaLaunchKernelEx(&cfg, plan_kernel<L>, p, a);
     return e == cudaSuccess ? NVFP4_OK : (int)e;
 }
 
@@ -328,40 +439,39 @@ int plan_ctas(long long copies) {
     return c;
 }
 
-template <int KIND, int NV>
+template <typename L>
 int launch_route(const RouteArgs& a, const PlanArgs& p, int dev, cudaStream_t st) {
-    // up to 256 tokens the sorting cluster chooses the experts itself, a token for each of its warps
+    // up to 256 tokens the sorting cluster chooses the experts itself, one round of tokens for each of its warps
     if (a.T <= 256) {
         int c = 1;
-        while (c < 8 && a.T > PLAN_WARPS * c) c *= 2;
-        return launch_plan<KIND, NV>(p, a, c, st);
+        while (c < 8 && a.T > PLAN_WARPS * L::PER_WARP * c) c *= 2;
+        return launch_plan<L>(p, a, c, st);
     }
-    int blocks = (a.T + 7) / 8;
+    int blocks = (a.T + 8 * L::PER_WARP - 1) / (8 * L::PER_WARP);
     if (blocks > 8 * sm_count(dev)) blocks = 8 * sm_count(dev);
-    route_kernel<KIND, NV><<<blocks, 256, 0, st>>>(a);
+    route_kernel<L><<<blocks, 256, 0, st>>>(a);
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return (int)e;
-    return launch_plan<-1, 1>(p, a, plan_ctas((long long)a.T * a.k), st);
+    return launch_plan<void>(p, a, plan_ctas((long long)a.T * a.k), st);
 }
 
-template <int KIND, int NV>
+template <typename L>
 int launch_backward(const RouteArgs& a, const float* dw, void* dlogits, int dev, cudaStream_t st) {
-    int blocks = (a.T + 7) / 8;
+    int blocks = (a.T + 8 * L::PER_WARP - 1) / (8 * L::PER_WARP);
     if (blocks > 8 * sm_count(dev)) blocks = 8 * sm_count(dev);
-    route_backward_kernel<KIND, NV><<<blocks, 256, 0, st>>>(a, dw, dlogits);
+    route_backward_kernel<L><<<blocks, 256, 0, st>>>(a, dw, dlogits);
     cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? NVFP4_OK : (int)e;
 }
 
-// f(KIND, NV) for the element type and the number of entries a lane holds
+// f(layout) for the element type and the number of experts
 template <int KIND, typename F>
 int by_width(int E, F&& f) {
-    if (E <= 32) return f(std::integral_constant<int, KIND>(), std::integral_constant<int, 1>());
-    if (E <= 64) return f(std::integral_constant<int, KIND>(), std::integral_constant<int, 2>());
-    if (E <= 128) return f(std::integral_constant<int, KIND>(), std::integral_constant<int, 4>());
-    if (E <= 256) return f(std::integral_constant<int, KIND>(), std::integral_constant<int, 8>());
-    if (E <= 512) return f(std::integral_constant<int, KIND>(), std::integral_constant<int, 16>());
-    return f(std::integral_constant<int, KIND>(), std::integral_constant<int, 32>());
+    if (E <= 64) return f(Layout<KIND, 8, 8>());
+    if (E <= 128) return f(Layout<KIND, 8, 16>());
+    if (E <= 256) return f(Layout<KIND, 16, 16>());
+    if (E <= 512) return f(Layout<KIND, 32, 16>());
+    return f(Layout<KIND, 32, 32>());
 }
 template <typename F>
 int by_kind(int kind, int E, F&& f) {
@@ -369,6 +479,8 @@ int by_kind(int kind, int E, F&& f) {
     if (kind == NVFP4_F16) return by_width<NVFP4_F16>(E, f);
     return by_width<NVFP4_BF16>(E, f);
 }
+// Whether every row of the logits starts on a 16-byte boundary.
+int rows_wide(const void* logits, int kind, long long ld) { return ((uintptr_t)logits | (unsigned long long)(ld * elem_bytes(kind))) % 16 == 0; }
 
 int check_route(int kind, long long ld, int T, int E, int k) {
     if (!kind_ok(kind)) return NVFP4_ERR_UNSUPPORTED;
@@ -386,10 +498,11 @@ extern "C" int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* of
                               void* source, void* stream) {
     if (!experts || !offsets || !tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
     if (T <= 0 || E <= 0 || k <= 0) return NVFP4_ERR_SHAPE;
+    if (k > MOE_MAX_CHOICES) return NVFP4_ERR_UNSUPPORTED;
     // (padded rows are counted in 32 bits: up to 127 more for every expert)
     if (E > MOE_MAX_EXPERTS || (long long)T * k + 128ll * E >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
     const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)rows, (int*)slots, (int*)source, T, E, k};
-    return launch_plan<-1, 1>(p, RouteArgs{}, plan_ctas((long long)T * k), (cudaStream_t)stream);
+    return launch_plan<void>(p, RouteArgs{}, plan_ctas((long long)T * k), (cudaStream_t)stream);
 }
 
 extern "C" int nvfp4_moe_route(const void* logits, int kind, long long ld, const void* mask, int T, int E, int k, int renormalize,
@@ -402,21 +515,24 @@ extern "C" int nvfp4_moe_route(const void* logits, int kind, long long ld, const
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;
-    const RouteArgs a{logits, ld, (const uint8_t*)mask, (float*)weights, (int*)experts, T, E, k, renormalize};
+    const RouteArgs a{logits, ld, (const uint8_t*)mask, (float*)weights, (int*)experts, T, E, k, renormalize,
+                      rows_wide(logits, kind, ld)};
     const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)rows, (int*)slots, (int*)source, T, E, k};
-    return by_kind(kind, E, [&](auto K, auto V) { return launch_route<decltype(K)::value, decltype(V)::value>(a, p, dev, (cudaStream_t)stream); });
+    return by_kind(kind, E, [&](auto layout) { return launch_route<decltype(layout)>(a, p, dev, (cudaStream_t)stream); });
 }
 
 extern "C" int nvfp4_moe_route_backward(const void* dweights, const void* logits, int kind, long long ld, const void* weights,
                                         const void* experts, int T, int E, int k, int renormalize, void* dlogits, void* stream) {
     if (!dweights || !logits || !weights || !experts || !dlogits) return NVFP4_ERR_NULL;
+    if ((uintptr_t)dlogits & 15) return NVFP4_ERR_ALIGN;
     int rc = check_route(kind, ld, T, E, k);
     if (rc) return rc;
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;
-    const RouteArgs a{logits, ld, nullptr, (float*)const_cast<void*>(weights), (int*)const_cast<void*>(experts), T, E, k, renormalize};
-    return by_kind(kind, E, [&](auto K, auto V) {
-        return launch_backward<decltype(K)::value, decltype(V)::value>(a, (const float*)dweights, dlogits, dev, (cudaStream_t)stream);
+    const RouteArgs a{logits, ld, nullptr, (float*)const_cast<void*>(weights), (int*)const_cast<void*>(experts), T, E, k, renormalize,
+                      rows_wide(logits, kind, ld)};
+    return by_kind(kind, E, [&](auto layout) {
+        return launch_backward<decltype(layout)>(a, (const float*)dweights, dlogits, dev, (cudaStream_t)stream);
     });
 }

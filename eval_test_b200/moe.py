@@ -30,25 +30,63 @@ MAX_EXPERTS, MAX_CHOICES = 1024, 32
 _KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
-class Plan(NamedTuple):
-    """How the copies of a batch are sorted; int32 tensors on the batch's device (``nvfp4_moe_plan``).  The tensors of one
-    plan share one allocation."""
-    offsets: torch.Tensor   # [E + 1] first row of each expert; offsets[E] rows are in use
-    tiles: torch.Tensor     # [E + 1] first 128-row tile of each expert
-    rows: torch.Tensor      # [T, k] row of a copy, -1: not routed
-    slots: torch.Tensor     # [T, k] row counted with every expert padded to whole tiles, -1: not routed
-    source: torch.Tensor    # [T * k] copy of a row, -1 behind the last
+class Plan:
+    """How the copies of a batch are sorted (``nvfp4_moe_plan``).  One int32 buffer on the batch's device holds its five
+    tables; the views are made when they are asked for (a call of the layer needs only their addresses)."""
+    __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "_at")
+
+    def __init__(self, num_tokens: int, top_k: int, num_experts: int, device: torch.device):
+        n = num_tokens * top_k
+        size = 2 * (num_experts + 1) + 3 * n
+        # (no copies: nothing is launched, and every expert starts at row 0)
+        self.buffer = torch.empty(size, dtype=torch.int32, device=device) if n else torch.zeros(size, dtype=torch.int32, device=device)
+        self.num_tokens, self.top_k, self.num_experts = num_tokens, top_k, num_experts
+        base, e, n = self.buffer.data_ptr(), 4 * (num_experts + 1), 4 * n
+        self._at = (base, base + e, base + 2 * e, base + 2 * e + n, base + 2 * e + 2 * n)
 
     @property
-    def num_experts(self) -> int:
-        return self.offsets.shape[0] - 1
+    def device(self) -> torch.device:
+        return self.buffer.device
+
+    @property
+    def num_copies(self) -> int:
+        return self.num_tokens * self.top_k
 
     @property
     def most_tiles(self) -> int:
         """128-row tiles that this many copies can fill at most, whatever their experts."""
-        copies, experts = self.source.shape[0], self.num_experts
-        active = min(copies, experts)
+        copies = self.num_tokens * self.top_k
+        active = min(copies, self.num_experts)
         return active + (copies - active) // 128
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        """[E + 1] first row of each expert; offsets[E] rows are in use."""
+        return self.buffer[:self.num_experts + 1]
+
+    @property
+    def tiles(self) -> torch.Tensor:
+        """[E + 1] first 128-row tile of each expert."""
+        return self.buffer[self.num_experts + 1:2 * (self.num_experts + 1)]
+
+    def _table(self, i: int) -> torch.Tensor:
+        return self.buffer.as_strided((self.num_tokens, self.top_k), (self.top_k, 1),
+                                      2 * (self.num_experts + 1) + i * self.num_tokens * self.top_k)
+
+    @property
+    def rows(self) -> torch.Tensor:
+        """[T, k] row of a copy, -1: not routed."""
+        return self._table(0)
+
+    @property
+    def slots(self) -> torch.Tensor:
+        """[T, k] row counted with every expert padded to whole tiles, -1: not routed."""
+        return self._table(1)
+
+    @property
+    def source(self) -> torch.Tensor:
+        """[T * k] copy of a row, -1 behind the last."""
+        return self.buffer[2 * (self.num_experts + 1) + 2 * self.num_tokens * self.top_k:]
 
 
 class Routing(NamedTuple):
@@ -61,11 +99,13 @@ def _matrix(t: torch.Tensor, name: str, rows: int | None = None, cols: int | Non
     """Checks ``[rows, cols]`` of a floating type whose rows are contiguous; returns the pitch in elements."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _KINDS):
         raise ValueError(f"{name}: expected a CUDA float32 / float16 / bfloat16 matrix")
-    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+    have_rows, have_cols = t.shape
+    if (rows is not None and have_rows != rows) or (cols is not None and have_cols != cols):
         raise ValueError(f"{name}: expected shape {(rows, cols)}, got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    pitch, step = t.stride()
+    if step != 1 and have_cols > 1:
         raise ValueError(f"{name}: the rows have to be contiguous, got strides {t.stride()}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return pitch if have_rows > 1 else have_cols
 
 
 def _choices(t: torch.Tensor, name: str, dtype: torch.dtype, shape=None) -> None:
@@ -93,12 +133,12 @@ def _call(entry: str, device: torch.device, *args) -> None:
         _lib.check(code, entry)
 
 
-def _new_plan(T: int, k: int, E: int, device) -> Plan:
-    n = T * k
-    make = torch.empty if n else torch.zeros             # (no tokens: no launch, every expert starts at row 0)
-    offsets, tiles, rows, slots, source = make(2 * (E + 1) + 3 * n, dtype=torch.int32, device=device).split(
-        [E + 1, E + 1, n, n, n])
-    return Plan(offsets, tiles, rows.view(T, k), slots.view(T, k), source)
+def _new_operand(rows: int, tile_rows: int, K: int, device):
+    """An operand ``[rows, K/2, 1]`` and the 6-D swizzled view of the scales of ``tile_rows`` rows, not initialised."""
+    packed = torch.empty((rows, K // 2, 1), dtype=torch.float4_e2m1fn_x2, device=device)
+    scales = torch.empty_strided((32, 4, tile_rows // 128, 4, K // 64, 1), F.permuted_strides(tile_rows, K),
+                                 dtype=torch.float8_e4m3fn, device=device)
+    return packed, scales
 
 
 def plan(experts: torch.Tensor, num_experts: int) -> Plan:
@@ -108,9 +148,11 @@ def plan(experts: torch.Tensor, num_experts: int) -> Plan:
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"num_experts: expected 1 to {MAX_EXPERTS}, got {num_experts}")
     T, k = experts.shape
-    p = _new_plan(T, k, num_experts, experts.device)
+    if k > MAX_CHOICES:
+        raise ValueError(f"experts: expected at most {MAX_CHOICES} choices for a token, got {k}")
+    p = Plan(T, k, num_experts, experts.device)
     if T * k:
-        _call("nvfp4_moe_plan", experts.device, experts.data_ptr(), T, num_experts, k, *(t.data_ptr() for t in p))
+        _call("nvfp4_moe_plan", experts.device, experts.data_ptr(), T, num_experts, k, *p._at)
     return p
 
 
@@ -134,10 +176,10 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torc
         _same_device(device, mask)
     weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
     experts = torch.empty((T, top_k), dtype=torch.int32, device=device)
-    p = _new_plan(T, top_k, E, device)
+    p = Plan(T, top_k, E, device)
     if T:
         _call("nvfp4_moe_route", device, logits.data_ptr(), _KINDS[logits.dtype], ld, None if mask is None else mask.data_ptr(),
-              T, E, top_k, int(renormalize), weights.data_ptr(), experts.data_ptr(), *(t.data_ptr() for t in p))
+              T, E, top_k, int(renormalize), weights.data_ptr(), experts.data_ptr(), *p._at)
     return Routing(weights, experts, p)
 
 
@@ -164,13 +206,13 @@ def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, weights: to
 
 def dispatch(x: torch.Tensor, plan: Plan) -> torch.Tensor:
     """``x`` [T, H] -> [T * k, H] of the same type: every token's row at the rows of its copies."""
-    T, k = plan.rows.shape
+    T, k = plan.num_tokens, plan.top_k
     ld = _matrix(x, "x", T)
     H = x.shape[1]
-    _same_device(x.device, plan.rows)
+    _same_device(x.device, plan)
     out = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
     if out.numel():
-        _call("nvfp4_moe_dispatch", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan.rows.data_ptr(), plan.offsets.data_ptr(), T,
+        _call("nvfp4_moe_dispatch", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[2], plan._at[0], T,
               plan.num_experts, k, H, out.data_ptr())
     return out
 
@@ -183,7 +225,7 @@ def dispatch_backward(grad_rows: torch.Tensor, plan: Plan) -> torch.Tensor:
 def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
     """``y`` [T * k, H], rows sorted by expert -> [T, H]: the sum of each token's rows times ``weights`` [T, k] (float32; none:
     the plain sum), in fp32, rounded once to ``dtype`` (default: that of ``y``).  Choices that are not routed add nothing."""
-    T, k = plan.rows.shape
+    T, k = plan.num_tokens, plan.top_k
     ld = _matrix(y, "y", T * k)
     H = y.shape[1]
     dtype = y.dtype if dtype is None else dtype
@@ -191,28 +233,28 @@ def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dt
         raise ValueError(f"dtype: expected float32, float16 or bfloat16, got {dtype}")
     if weights is not None:
         _choices(weights, "weights", torch.float32, (T, k))
-    _same_device(y.device, plan.rows, weights)
+    _same_device(y.device, plan, weights)
     make = torch.empty if k else torch.zeros
     out = make((T, H), dtype=dtype, device=y.device)
     if out.numel() and k:
         _call("nvfp4_moe_combine", y.device, y.data_ptr(), _KINDS[y.dtype], ld, None if weights is None else weights.data_ptr(),
-              plan.rows.data_ptr(), T, k, H, out.data_ptr(), _KINDS[dtype])
+              plan._at[2], T, k, H, out.data_ptr(), _KINDS[dtype])
     return out
 
 
 def combine_backward(grad_out: torch.Tensor, y: torch.Tensor, plan: Plan, weights: torch.Tensor):
     """Gradients of ``combine`` with weights: ``grad_out`` [T, H] -> (that of ``y``, same type, rows that belong to no copy 0;
     that of ``weights`` [T, k], 0 where a choice is not routed)."""
-    T, k = plan.rows.shape
+    T, k = plan.num_tokens, plan.top_k
     ldo, ld = _matrix(grad_out, "grad_out", T), _matrix(y, "y", T * k, grad_out.shape[1])
     H = y.shape[1]
     _choices(weights, "weights", torch.float32, (T, k))
-    _same_device(y.device, grad_out, plan.rows, weights)
+    _same_device(y.device, grad_out, plan, weights)
     dy = torch.empty((T * k, H), dtype=y.dtype, device=y.device)
     dw = (torch.empty if H else torch.zeros)((T, k), dtype=torch.float32, device=y.device)
     if dy.numel():
         _call("nvfp4_moe_combine_backward", y.device, grad_out.data_ptr(), _KINDS[grad_out.dtype], ldo, y.data_ptr(), _KINDS[y.dtype],
-              ld, weights.data_ptr(), plan.rows.data_ptr(), plan.offsets.data_ptr(), T, plan.num_experts, k, H, dy.data_ptr(),
+              ld, weights.data_ptr(), plan._at[2], plan._at[0], T, plan.num_experts, k, H, dy.data_ptr(),
               dw.data_ptr())
     return dy, dw
 
@@ -221,24 +263,22 @@ def dispatch_nvfp4(x: torch.Tensor, plan: Plan):
     """``dispatch`` with the rows quantised as ``quantize.quantize_operand`` does: ``x`` [T, K] -> (operand
     ``[T * k, K/2, 1]`` float4_e2m1fn_x2, 6-D swizzled scales of the experts' 128-row tiles, ``plan.most_tiles`` of them).
     Scale bytes of rows that do not exist are not written.  K is a multiple of 64."""
-    T, k = plan.rows.shape
+    T, k = plan.num_tokens, plan.top_k
     ld = _matrix(x, "x", T)
     K = x.shape[1]
     if K % 64 or not K:
         raise ValueError(f"x: the width has to be a multiple of 64, got {K}")
-    _same_device(x.device, plan.rows)
-    packed = torch.empty((1, T * k, K // 2), dtype=torch.uint8, device=x.device)
-    rows = plan.most_tiles * 128
-    scales = torch.empty(F.sf_buffer_bytes(rows, K), dtype=torch.uint8, device=x.device)
+    _same_device(x.device, plan)
+    packed, scales = _new_operand(T * k, plan.most_tiles * 128, K, x.device)
     if T * k:
-        _call("nvfp4_moe_dispatch_nvfp4", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan.rows.data_ptr(), plan.slots.data_ptr(),
-              plan.offsets.data_ptr(), T, plan.num_experts, k, K, packed.data_ptr(), scales.data_ptr())
-    return F.batch_last(packed).view(torch.float4_e2m1fn_x2), F.permuted_view(scales, rows, K, 1)
+        _call("nvfp4_moe_dispatch_nvfp4", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[2], plan._at[3],
+              plan._at[0], T, plan.num_experts, k, K, packed.data_ptr(), scales.data_ptr())
+    return packed, scales
 
 
 def _products(a, sfa, weights, plan: Plan, alpha):
     """Checks the operands of an expert product -> (pointers in the C order, alphas pointer, alpha, R, E, N, K, device)."""
-    R, E = plan.source.shape[0], plan.num_experts
+    R, E = plan.num_copies, plan.num_experts
     device = a.device
     if a.dim() != 3 or not a.is_cuda:
         raise ValueError("a: expected the CUDA operand [T * k, K/2, 1] that dispatch_nvfp4 returns")
@@ -250,14 +290,14 @@ def _products(a, sfa, weights, plan: Plan, alpha):
     ptrs = [_args.operand_ptr(a, R, K // 2, 1, "a"), _args.scales_ptr(sfa, plan.most_tiles * 128, K, 1, "sfa")]
     for i in range(0, len(weights), 2):
         ptrs += [_args.operand_ptr(weights[i], N, K // 2, E, "b"), _args.scales_ptr(weights[i + 1], N, K, E, "sfb")]
-    _same_device(device, sfa, *weights, plan.rows)
+    _same_device(device, sfa, *weights, plan)
     alphas = None
     if isinstance(alpha, torch.Tensor):
         if alpha.dtype != torch.float32 or alpha.shape != (E,) or not alpha.is_contiguous():
             raise ValueError(f"alpha: expected a number or a contiguous float32 tensor of shape {(E,)}")
         _same_device(device, alpha)
         alphas, alpha = alpha.data_ptr(), 1.0
-    return ptrs + [plan.offsets.data_ptr(), plan.tiles.data_ptr(), alphas], float(alpha), R, E, N, K, device
+    return ptrs + [plan._at[0], plan._at[1], alphas], float(alpha), R, E, N, K, device
 
 
 def expert_gemm(a, sfa, b, sfb, plan: Plan, alpha=1.0) -> torch.Tensor:
@@ -285,9 +325,7 @@ def expert_dual_gemm_nvfp4(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0):
     """``expert_dual_gemm`` with its rows quantised to NVFP4, bit for bit what quantising the fp16 rows gives -> (operand
     ``[T * k, N/2, 1]``, 6-D scales): ``a`` and ``sfa`` of the next product of the same plan."""
     ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
-    packed = torch.empty((1, R, N // 2), dtype=torch.uint8, device=device)
-    rows = plan.most_tiles * 128
-    scales = torch.empty(F.sf_buffer_bytes(rows, N), dtype=torch.uint8, device=device)
+    packed, scales = _new_operand(R, plan.most_tiles * 128, N, device)
     if R:
         _call("nvfp4_moe_dual_gemm_nvfp4", device, *ptrs, packed.data_ptr(), scales.data_ptr(), R, E, N, K, alpha)
-    return F.batch_last(packed).view(torch.float4_e2m1fn_x2), F.permuted_view(scales, rows, N, 1)
+    return packed, scales

@@ -135,7 +135,7 @@ int nvfp4_quantize_bf16(const void* x, void* packed, void* sf_sw, int rows, int 
 
 /* ---------------------------------------------------------------------------------------------------------------
  * Mixture-of-experts layer around the products: router, tokens sorted by expert and back, the experts' products.
- * T tokens choose k of E experts (E <= 1024, k <= 32 in the router); copy i = t*k + j is choice j of token t.  The copies
+ * T tokens choose k of E experts (E <= 1024, k <= 32); copy i = t*k + j is choice j of token t.  The copies
  * are sorted stably by expert into R = T*k rows.  The group sizes stay on the device, so a whole layer can be captured
  * into a graph (eval/nvfp4_grouped_gemm/reference.py:137-201 takes them as a host list).  An expert id outside [0, E)
  * means "not routed": the copy has no row.  No entry point keeps a workspace: what it needs is an argument.
@@ -148,7 +148,7 @@ enum { NVFP4_F32 = 0, NVFP4_F16 = 1, NVFP4_BF16 = 2 };
  *   rows    [T][k] row of a copy, -1: none
  *   slots   [T][k] 128 * tile + row in the tile: where the scales of the copy's row are, -1: none
  *   source  [T*k]  copy of a row, -1 behind the last one
- * all int32.  T, E, k > 0. */
+ * all int32.  T, E, k > 0, k <= 32. */
 int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* rows, void* slots,
                    void* source, void* stream);
 

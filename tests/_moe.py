@@ -28,7 +28,9 @@ def plan_ref(experts: torch.Tensor, E: int):
 
 
 def check_plan(plan, experts, E):
-    for name, got, want in zip(plan._fields, plan, plan_ref(experts, E)):
+    assert (plan.num_tokens, plan.top_k, plan.num_experts) == (*experts.shape, E)
+    for name, want in zip(("offsets", "tiles", "rows", "slots", "source"), plan_ref(experts, E)):
+        got = getattr(plan, name)
         assert got.dtype == torch.int32 and torch.equal(got.cpu().long(), want), name
 
 

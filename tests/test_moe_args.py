@@ -10,6 +10,7 @@ def test_c_entries_reject_bad_arguments(lib):
     assert lib.nvfp4_moe_plan(P, 0, 4, 2, *plan, None) == -2
     assert lib.nvfp4_moe_plan(P, 4, 0, 2, *plan, None) == -2
     assert lib.nvfp4_moe_plan(P, 4, 1025, 2, *plan, None) == -6
+    assert lib.nvfp4_moe_plan(P, 4, 64, 33, *plan, None) == -6
     assert lib.nvfp4_moe_plan(P, 1 << 30, 4, 2, *plan, None) == -6       # copies are counted in 32 bits
     route = lambda kind=0, ld=8, T=4, E=8, k=2, logits=P: lib.nvfp4_moe_route(  # noqa: E731
         logits, kind, ld, None, T, E, k, 1, P, P, *plan, None)
@@ -17,8 +18,8 @@ def test_c_entries_reject_bad_arguments(lib):
     assert route(kind=3) == -6
     assert route(T=0) == -2 and route(E=0) == -2 and route(k=0) == -2 and route(k=9) == -2 and route(ld=-1) == -2
     assert route(E=1025) == -6 and route(E=64, k=33) == -6
-    back = lambda kind=0, k=2, dw=P: lib.nvfp4_moe_route_backward(dw, P, kind, 8, P, P, 4, 8, k, 1, P, None)  # noqa: E731
-    assert back(dw=None) == -1 and back(kind=-1) == -6 and back(k=9) == -2
+    back = lambda kind=0, k=2, dw=P, out=P: lib.nvfp4_moe_route_backward(dw, P, kind, 8, P, P, 4, 8, k, 1, out, None)  # noqa: E731
+    assert back(dw=None) == -1 and back(out=8) == -5 and back(kind=-1) == -6 and back(k=9) == -2
     disp = lambda x=P, kind=0, T=4, H=8, xs=P, ld=8: lib.nvfp4_moe_dispatch(x, kind, ld, P, P, T, 8, 2, H, xs, None)  # noqa: E731
     assert disp(x=None) == -1 and disp(kind=9) == -6 and disp(T=0) == -2 and disp(H=0) == -2 and disp(T=1 << 30) == -6
     comb = lambda y=P, kind=0, ok=0, k=2: lib.nvfp4_moe_combine(y, kind, 8, None, P, 4, k, 8, P, ok, None)  # noqa: E731
@@ -45,7 +46,7 @@ def test_python_entries_take_cuda_tensors_of_the_documented_types():
         moe.route(x, 2)
     with pytest.raises(ValueError, match="CUDA"):
         moe.plan(torch.zeros((4, 2), dtype=torch.int32), 8)
-    p = moe.Plan(*(torch.zeros(s, dtype=torch.int32) for s in ((9,), (9,), (4, 2), (4, 2), (8,))))
+    p = moe.Plan(4, 2, 8, torch.device("cpu"))
     for f in (moe.dispatch, moe.dispatch_nvfp4, moe.combine, moe.dispatch_backward):
         with pytest.raises(ValueError, match="CUDA"):
             f(x, p)
@@ -65,6 +66,6 @@ def test_most_tiles_bounds_every_distribution():
         return sum((c + 127) // 128 for c in counts)
 
     for copies, E in ((0, 3), (1, 3), (2, 3), (130, 1), (256, 2), (257, 2), (400, 3), (513, 3)):
-        p = moe.Plan(torch.zeros(E + 1), None, None, None, torch.zeros(copies))
+        p = moe.Plan(copies, 1, E, torch.device("cpu"))
         reached = max(tiles((*c, copies - sum(c))) for c in product(range(copies + 1), repeat=E - 1) if sum(c) <= copies)
         assert p.most_tiles == reached, (copies, E)

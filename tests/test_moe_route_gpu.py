@@ -181,5 +181,7 @@ def test_refusals():
         moe.plan(ids, 0)
     with pytest.raises(ValueError, match="experts"):
         moe.plan(ids.long(), 4)
+    with pytest.raises(ValueError, match="choices"):
+        moe.plan(torch.zeros((4, 33), dtype=torch.int32, device="cuda"), 64)
     with pytest.raises(ValueError, match="weights"):
         moe.route_backward(torch.zeros((4, 2), device="cuda"), l, torch.zeros((4, 3), device="cuda"), ids)
