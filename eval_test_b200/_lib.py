@@ -78,8 +78,10 @@ def load() -> ctypes.CDLL:
     for q in (lib.nvfp4_quantize_f32, lib.nvfp4_quantize_f16, lib.nvfp4_quantize_bf16):
         q.argtypes = [vp, vp, vp, i, i, i, vp]
     ll = ctypes.c_longlong
-    lib.nvfp4_moe_plan.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, vp]
-    lib.nvfp4_moe_route.argtypes = [vp, i, ll, vp, i, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.nvfp4_moe_plan.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, vp, vp]
+    lib.nvfp4_moe_plan_scratch.argtypes = [i, i, i]
+    lib.nvfp4_moe_plan_scratch.restype = ll
+    lib.nvfp4_moe_route.argtypes = [vp, i, ll, vp, i, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp]
     lib.nvfp4_moe_route_backward.argtypes = [vp, vp, i, ll, vp, vp, i, i, i, i, vp, vp]
     lib.nvfp4_moe_dispatch.argtypes = [vp, i, ll, vp, vp, i, i, i, i, vp, vp]
     lib.nvfp4_moe_combine.argtypes = [vp, i, ll, vp, vp, i, i, i, vp, i, vp]

@@ -113,6 +113,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         tmem_base = tmem_base_slot;
     }
 
+    if (EXPERTS) {
+        pdl_wait();
+        pdl_launch();
+    }
     // (experts: the tile count comes from the plan; a launch has enough CTAs for the most there can be)
     const int total_tiles = EXPERTS ? __ldg(p.experts.tiles + p.experts.E) * (p.N / BN) : p.total_tiles;
 
@@ -399,9 +403,13 @@ static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
     }
     if (p.total_tiles <= 0) return NVFP4_OK;
     const int grid = p.total_tiles < sm_count(dev) ? p.total_tiles : sm_count(dev);
-    kern<<<grid, GEMM_THREADS, SMEM, stream>>>(ta, tb, tb2, gm, p);
-    e = cudaGetLastError();
-    return e == cudaSuccess ? NVFP4_OK : (int)e;
+    if constexpr (EXPERTS) {
+        return launch_dependent(kern, grid, GEMM_THREADS, SMEM, 0, stream, ta, tb, tb2, gm, p);
+    } else {
+        kern<<<grid, GEMM_THREADS, SMEM, stream>>>(ta, tb, tb2, gm, p);
+        e = cudaGetLastError();
+        return e == cudaSuccess ? NVFP4_OK : (int)e;
+    }
 }
 
 static int check_common(const void* const* ptrs, int nptr, int M, int N, int K, int L) {

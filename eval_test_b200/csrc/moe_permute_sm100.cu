@@ -84,6 +84,8 @@ template <int BYTES, int U>
 __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* __restrict__ x, long long ld, void* __restrict__ xs,
                                                        int row_vecs, const PermuteArgs p) {
     using V = typename Bits<BYTES>::type;
+    pdl_wait();
+    pdl_launch();
     V* out = reinterpret_cast<V*>(xs);
     for (Pieces<U, false> w(p, nullptr, row_vecs); w.more(); w.next()) {
         const V* src = reinterpret_cast<const V*>(x + w.t * ld);
@@ -107,6 +109,8 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* __restrict
 template <typename TI, typename TO, int VN, int KU, int U, bool WEIGHTED>
 __global__ void __launch_bounds__(256, U == 2 ? 3 : 4) combine_kernel(const TI* __restrict__ y, unsigned pitch, const float* __restrict__ weights,
                                                          TO* __restrict__ out, int row_vecs, const PermuteArgs p) {
+    pdl_wait();
+    pdl_launch();
     for (Pieces<U, WEIGHTED> w(p, weights, row_vecs); w.more(); w.next()) {
         float acc[U][VN] = {};
         const char* at = reinterpret_cast<const char*>(y + (size_t)w.c * VN);
@@ -151,6 +155,8 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* __re
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int in_group = threadIdx.x % GROUP;
     constexpr int PER_BLOCK = 256 / GROUP;
+    pdl_wait();
+    pdl_launch();
     const unsigned out_pitch = (unsigned)p.H * (unsigned)sizeof(TI);
     for (long long t = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / GROUP; t < p.T; t += (long long)gridDim.x * PER_BLOCK) {
         const TO* d = dout + t * ldo;
@@ -233,6 +239,8 @@ __global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* __restr
                                                              uint8_t* __restrict__ codes, uint8_t* __restrict__ sf_sw,
                                                              const PermuteArgs p) {
     using T = typename ElemOf<KIND>::type;
+    pdl_wait();
+    pdl_launch();
     const int units = p.H / 32;
     const int lane = threadIdx.x & 31;
     const long long n = (long long)p.T * units, step = (long long)gridDim.x * blockDim.x;
@@ -288,11 +296,6 @@ int current_device(int* dev) {
     return *dev < 64 ? NVFP4_OK : NVFP4_ERR_UNSUPPORTED;
 }
 
-int launched() {
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? NVFP4_OK : (int)e;
-}
-
 int check_sizes(int T, int k, int H, long long ld) {
     if (T <= 0 || k <= 0 || H <= 0 || ld < 0) return NVFP4_ERR_SHAPE;
     if (k > MOE_MAX_CHOICES || (long long)T * k >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
@@ -338,8 +341,7 @@ extern "C" int nvfp4_moe_dispatch(const void* x, int kind, long long ld, const v
         constexpr int B = decltype(bytes)::value, U = decltype(u)::value;
         const long long warps = (long long)T * ((row_vecs + 32 * U - 1) / (32 * U));
         if (warps >= (1ll << 31)) return (int)NVFP4_ERR_UNSUPPORTED;
-        dispatch_kernel<B, U><<<grid_for(32 * warps, dev), 256, 0, st>>>((const uint8_t*)x, ld * size, xs, row_vecs, p);
-        return launched();
+        return launch_dependent(dispatch_kernel<B, U>, grid_for(32 * warps, dev), 256, 0, 0, st, (const uint8_t*)x, ld * size, xs, row_vecs, p);
     };
     auto go_bytes = [&](auto bytes) {
         return spread(T, row_vecs, dev) ? go(bytes, std::integral_constant<int, 1>()) : go(bytes, std::integral_constant<int, 4>());
@@ -379,11 +381,8 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
                 if (warps >= (1ll << 31)) return (int)NVFP4_ERR_UNSUPPORTED;
                 const int grid = grid_for(32 * warps, dev);
                 const unsigned pitch = (unsigned)(ld * sizeof(TI));
-                if (weights)
-                    combine_kernel<TI, TO, N, KU, U, true><<<grid, 256, 0, st>>>((const TI*)y, pitch, (const float*)weights, (TO*)out, row_vecs, p);
-                else
-                    combine_kernel<TI, TO, N, KU, U, false><<<grid, 256, 0, st>>>((const TI*)y, pitch, nullptr, (TO*)out, row_vecs, p);
-                return launched();
+                return launch_dependent(weights ? combine_kernel<TI, TO, N, KU, U, true> : combine_kernel<TI, TO, N, KU, U, false>, grid,
+                                        256, 0, 0, st, (const TI*)y, pitch, (const float*)weights, (TO*)out, row_vecs, p);
             };
             using std::integral_constant;
             auto go_width = [&](auto vn) {
@@ -426,10 +425,10 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
             const bool warp = row_vecs <= 128;
             const int grid = grid_for((long long)T * (warp ? 32 : 256), dev);
             auto go = [&](auto vn, auto group, auto ku, auto u) {
-                combine_backward_kernel<TI, TO, decltype(vn)::value, decltype(group)::value, decltype(ku)::value, decltype(u)::value>
-                    <<<grid, 256, 0, st>>>((const TO*)dout, ldo, (const TI*)y, (unsigned)(ld * sizeof(TI)), (const float*)weights, (TI*)dy,
-                                           (float*)dweights, row_vecs, p);
-                return launched();
+                return launch_dependent(
+                    combine_backward_kernel<TI, TO, decltype(vn)::value, decltype(group)::value, decltype(ku)::value, decltype(u)::value>,
+                    grid, 256, 0, 0, st, (const TO*)dout, ldo, (const TI*)y, (unsigned)(ld * sizeof(TI)), (const float*)weights, (TI*)dy,
+                    (float*)dweights, row_vecs, p);
             };
             using std::integral_constant;
             auto go_group = [&](auto vn, auto group) {
@@ -459,10 +458,8 @@ extern "C" int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, c
     const PermuteArgs p{(const int*)rows, (const int*)offsets + E, T, k, K};
     const int grid = grid_for((long long)T * (K / 32), dev);
     cudaStream_t st = (cudaStream_t)stream;
-    switch (kind) {
-        case NVFP4_F32: dispatch_quant_kernel<NVFP4_F32><<<grid, 256, 0, st>>>(x, ld, (const int*)slots, (uint8_t*)packed, (uint8_t*)sf_sw, p); break;
-        case NVFP4_F16: dispatch_quant_kernel<NVFP4_F16><<<grid, 256, 0, st>>>(x, ld, (const int*)slots, (uint8_t*)packed, (uint8_t*)sf_sw, p); break;
-        default: dispatch_quant_kernel<NVFP4_BF16><<<grid, 256, 0, st>>>(x, ld, (const int*)slots, (uint8_t*)packed, (uint8_t*)sf_sw, p); break;
-    }
-    return launched();
+    auto kernel = kind == NVFP4_F32   ? dispatch_quant_kernel<NVFP4_F32>
+                  : kind == NVFP4_F16 ? dispatch_quant_kernel<NVFP4_F16>
+                                      : dispatch_quant_kernel<NVFP4_BF16>;
+    return launch_dependent(kernel, grid, 256, 0, 0, st, x, ld, (const int*)slots, (uint8_t*)packed, (uint8_t*)sf_sw, p);
 }

@@ -159,6 +159,8 @@ __device__ __forceinline__ void route_token(const RouteArgs& a, int t, int in_gr
 
 template <typename L>
 __global__ void __launch_bounds__(256) route_kernel(const RouteArgs a) {
+    pdl_wait();
+    pdl_launch();
     const int lane = threadIdx.x & 31;
     const int warps = gridDim.x * (blockDim.x >> 5);
     for (int t = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * L::PER_WARP; t < a.T; t += warps * L::PER_WARP)
@@ -170,6 +172,8 @@ template <typename L>
 __global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a, const float* __restrict__ dw, void* dlogits) {
     using T = typename L::T;
     constexpr int G = L::G, NV = L::NV;
+    pdl_wait();
+    pdl_launch();
     const int lane = threadIdx.x & 31, in_group = lane % G;
     const int warps = gridDim.x * (blockDim.x >> 5);
     for (int t0 = (blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * L::PER_WARP; t0 < a.T; t0 += warps * L::PER_WARP) {
@@ -260,10 +264,13 @@ struct PlanArgs {
     int* rows;                 // [T][k] sorted row of a copy, -1: none
     int* slots;                // [T][k] the row counted with every expert padded to whole tiles, -1: none
     int* source;               // [T*k] copy of a sorted row, -1 behind the last
+    uint32_t* counts;          // [PLAN_BLOCKS][E] copies of a block: the spread form only
     int T, E, k;
 };
 
 constexpr int PLAN_WARPS = 32;
+constexpr int PLAN_BLOCKS = 128;   // of the spread form
+constexpr long long PLAN_CLUSTER_MOST = 16384;   // copies that are sorted by one cluster
 constexpr int PLAN_AHEAD = 8;      // rounds of 32 copies whose ids a warp has in flight
 
 __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t cluster_addr) {
@@ -289,28 +296,55 @@ __device__ __forceinline__ uint32_t same_key(int key, int bits) {
     return same;
 }
 
-// The whole sort is ONE cluster: every warp owns a contiguous run of tokens, counts its copies per expert, the counts
-// are summed over the warps of a CTA in its shared memory and over the CTAs through distributed shared memory, and a
-// second walk over the same copies hands out the rows in order.  No global scratch, no atomics, so the order is that
-// of the copies and a graph can replay it beside any other.  L: the warps choose their tokens' experts first, in that
-// layout (few tokens: one launch for router and plan); void: the choices are given.
-template <typename L>
+// The tokens of a warp of the plan: every warp of every block owns a contiguous run.
+__device__ __forceinline__ int first_token(int T, int warps, long long warp) {
+    const int per = (T + warps - 1) / warps;
+    return (int)min((long long)T, warp * per);
+}
+
+// Copies per expert of each block of the spread form (any order: they are only counted).
+__global__ void __launch_bounds__(PLAN_WARPS * 32) plan_count_kernel(const PlanArgs p) {
+    __shared__ uint32_t count[MOE_MAX_EXPERTS];
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) count[e] = 0;
+    __syncthreads();
+    pdl_wait();
+    pdl_launch();
+    const int begin = first_token(p.T, PLAN_BLOCKS * PLAN_WARPS, (long long)blockIdx.x * PLAN_WARPS) * p.k;
+    const int end = first_token(p.T, PLAN_BLOCKS * PLAN_WARPS, (long long)(blockIdx.x + 1) * PLAN_WARPS) * p.k;
+    for (int i = begin + threadIdx.x; i < end; i += blockDim.x) {
+        const int e = p.experts[i];
+        if ((unsigned)e < (unsigned)p.E) atomicAdd(count + e, 1u);
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < p.E; e += blockDim.x) p.counts[blockIdx.x * p.E + e] = count[e];
+}
+
+// Every warp counts its copies per expert, the counts are summed over the warps of a block in its shared memory and
+// over the blocks, and a second walk over the same copies hands out the rows in order.  No atomics decide an order, so
+// it is that of the copies, and nothing is left behind between calls.
+//   one cluster (SPREAD = false): the blocks exchange their counts through distributed shared memory.  One launch, no
+//     scratch; L: the warps choose their tokens' experts first, in that layout (few tokens: router and plan in one);
+//   spread: PLAN_BLOCKS blocks on as many SMs, whose counts plan_count_kernel has left in memory.
+// 131072 copies, 64 experts: 25.8 us in a cluster of 8 (what bounds it is the scattered stores and the votes of eight
+// SMs), SPREAD_MEASURED us spread over 128 blocks, the counting included; up to 16384 copies the one launch is faster.
+template <typename L, bool SPREAD>
 __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs p, const RouteArgs a) {
     extern __shared__ uint32_t plan_smem[];
     uint32_t* hist = plan_smem;                         // [PLAN_WARPS][E]
-    uint32_t* total = hist + PLAN_WARPS * p.E;          // [E] copies of this CTA
-    uint32_t* base = total + p.E;                       // [E] first row of this CTA's copies
+    uint32_t* total = hist + PLAN_WARPS * p.E;          // [E] copies of this block; spread: of all blocks
+    uint32_t* base = total + p.E;                       // [E] first row of this block's copies
     int* shift = reinterpret_cast<int*>(base + p.E);    // [E] slot - row of the expert
     __shared__ uint32_t warp_total[2][PLAN_WARPS];
     __shared__ uint32_t live_rows;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = cluster_ctarank(), ctas = cluster_size();
-    const int per = (p.T + (int)ctas * PLAN_WARPS - 1) / ((int)ctas * PLAN_WARPS);
+    const uint32_t rank = SPREAD ? blockIdx.x : cluster_ctarank(), ctas = SPREAD ? gridDim.x : cluster_size();
     const long long g = (long long)rank * PLAN_WARPS + warp;
-    const int t0 = (int)min((long long)p.T, g * per), t1 = (int)min((long long)p.T, (g + 1) * per);
+    const int t0 = first_token(p.T, (int)ctas * PLAN_WARPS, g), t1 = first_token(p.T, (int)ctas * PLAN_WARPS, g + 1);
     const int begin = t0 * p.k, end = t1 * p.k;         // (T * k < 2^31: checked by the caller)
 
-    for (int i = threadIdx.x; i < PLAN_WARPS * p.E; i += blockDim.x) hist[i] = 0;
+    for (int i = threadIdx.x; i < (PLAN_WARPS + 2) * p.E; i += blockDim.x) hist[i] = 0;
+    pdl_wait();
+    pdl_launch();
     if constexpr (!std::is_void_v<L>) {
         for (int t = t0; t < t1; t += L::PER_WARP) {
             const int tg = t + lane / L::G;
@@ -318,9 +352,25 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
         }
     }
     __syncthreads();
+    if (SPREAD) {
+        // total: all blocks, base: the blocks before this one; the block's warps take a share of the blocks each
+        const int wide = (p.E + 31) / 32 * 32, shares = PLAN_WARPS * 32 / wide;
+        const int share = threadIdx.x / wide, e = threadIdx.x - share * wide;
+        if (share < shares && e < p.E) {
+            uint32_t all = 0, before = 0;
+#pragma unroll 8
+            for (uint32_t b = share; b < ctas; b += shares) {
+                const uint32_t c = p.counts[b * p.E + e];
+                all += c;
+                before += b < rank ? c : 0;
+            }
+            atomicAdd(total + e, all);
+            atomicAdd(base + e, before);
+        }
+    }
     uint32_t* own = hist + warp * p.E;
     const int bits = 32 - __clz(p.E);                   // keys 0 .. E
-    // (eight loads in flight: one after the other they were most of the kernel's time)
+    // (eight loads in flight)
     for (int i0 = begin; i0 < end; i0 += 32 * PLAN_AHEAD) {
         int ids[PLAN_AHEAD];
 #pragma unroll
@@ -338,23 +388,31 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     __syncthreads();
     for (int e = threadIdx.x; e < p.E; e += blockDim.x) {
         uint32_t run = 0;
+#pragma unroll 8
         for (int w = 0; w < PLAN_WARPS; w++) {
             const uint32_t c = hist[w * p.E + e];
             hist[w * p.E + e] = run;
             run += c;
         }
-        total[e] = run;
+        if (!SPREAD) total[e] = run;
     }
-    cluster_sync_all();
-    // thread e: the expert's copies in all CTAs, in the CTAs before this one; then its first row and first tile
+    // thread e: the expert's copies in all blocks, in the blocks before this one; then its first row and first tile
     // (MOE_MAX_EXPERTS = threads of the block)
     uint32_t count = 0, before = 0;
-    if (threadIdx.x < p.E) {
-        const uint32_t addr = smem_u32(total + threadIdx.x);
-        for (uint32_t r = 0; r < ctas; r++) {
-            const uint32_t c = ld_cluster_u32(mapa_shared(addr, r));
-            before += r < rank ? c : 0;
-            count += c;
+    if (SPREAD) {
+        if (threadIdx.x < p.E) { count = total[threadIdx.x]; before = base[threadIdx.x]; }
+    } else if (ctas == 1) {
+        if (threadIdx.x < p.E) count = total[threadIdx.x];
+    } else {
+        cluster_sync_all();
+        if (threadIdx.x < p.E) {
+            const uint32_t addr = smem_u32(total + threadIdx.x);
+#pragma unroll 8
+            for (uint32_t r = 0; r < ctas; r++) {
+                const uint32_t c = ld_cluster_u32(mapa_shared(addr, r));
+                before += r < rank ? c : 0;
+                count += c;
+            }
         }
     }
     const uint32_t ntiles = (count + 127) / 128;
@@ -377,8 +435,9 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
             if (rank == 0) { p.offsets[p.E] = (int)(row0 + count); p.tiles[p.E] = (int)(tile0 + ntiles); }
         }
     }
-    // also: no CTA leaves while a peer may still read its counts
-    cluster_sync_all();
+    // also: no CTA of a cluster leaves while a peer may still read its counts
+    if (SPREAD || ctas == 1) __syncthreads();
+    else cluster_sync_all();
     for (int i0 = begin; i0 < end; i0 += 32 * PLAN_AHEAD) {
         int ids[PLAN_AHEAD];
 #pragma unroll
@@ -405,7 +464,7 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     for (long long i = (long long)live_rows + rank * blockDim.x + threadIdx.x; i < n; i += (long long)ctas * blockDim.x) p.source[i] = -1;
 }
 
-template <typename L>
+template <typename L, bool SPREAD>
 int launch_plan(const PlanArgs& p, const RouteArgs& a, int ctas, cudaStream_t st) {
     static bool configured[64] = {};
     int dev = 0;
@@ -414,29 +473,31 @@ int launch_plan(const PlanArgs& p, const RouteArgs& a, int ctas, cudaStream_t st
     if (dev >= 64) return NVFP4_ERR_UNSUPPORTED;
     constexpr size_t most = (size_t)(PLAN_WARPS + 3) * MOE_MAX_EXPERTS * 4;
     if (!configured[dev]) {
-        e = cudaFuncSetAttribute(plan_kernel<L>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        e = cudaFuncSetAttribute(plan_kernel<L, SPREAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (e != cudaSuccess) return (int)e;
         configured[dev] = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(PLAN_WARPS * 32);
-    cfg.dynamicSmemBytes = (size_t)(PLAN_WARPS + 3) * p.E * 4;
-    cfg.stream = st;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ctas; attr.val.clusterDim.y = 1; attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, plan_kernel<L>, p, a);
-    return e == cudaSuccess ? NVFP4_OK : (int)e;
+    return launch_dependent(plan_kernel<L, SPREAD>, ctas, PLAN_WARPS * 32, (size_t)(PLAN_WARPS + 3) * p.E * 4, SPREAD ? 0 : ctas, st, p, a);
 }
 
-// CTAs of the sorting cluster: one for up to 1024 copies, then up to the eight that every device can place.
-int plan_ctas(long long copies) {
+// The plan of choices that are in memory.  In a cluster: one CTA for up to 1024 copies, then up to the eight that every
+// device can place.
+int plan_choices(const PlanArgs& p, cudaStream_t st) {
+    const long long copies = (long long)p.T * p.k;
+    if (copies > PLAN_CLUSTER_MOST) {
+        int rc = launch_dependent(plan_count_kernel, PLAN_BLOCKS, PLAN_WARPS * 32, 0, 0, st, p);
+        return rc ? rc : launch_plan<void, true>(p, RouteArgs{}, PLAN_BLOCKS, st);
+    }
     int c = 1;
     while (c < 8 && copies > 1024ll * c) c *= 2;
-    return c;
+    return launch_plan<void, false>(p, RouteArgs{}, c, st);
+}
+
+// Blocks of eight warps for `a.T` tokens, at most eight on an SM.
+template <typename L>
+int token_blocks(const RouteArgs& a, int dev) {
+    const int blocks = (a.T + 8 * L::PER_WARP - 1) / (8 * L::PER_WARP);
+    return blocks < 8 * sm_count(dev) ? blocks : 8 * sm_count(dev);
 }
 
 template <typename L>
@@ -445,23 +506,10 @@ int launch_route(const RouteArgs& a, const PlanArgs& p, int dev, cudaStream_t st
     if (a.T <= 256) {
         int c = 1;
         while (c < 8 && a.T > PLAN_WARPS * L::PER_WARP * c) c *= 2;
-        return launch_plan<L>(p, a, c, st);
+        return launch_plan<L, false>(p, a, c, st);
     }
-    int blocks = (a.T + 8 * L::PER_WARP - 1) / (8 * L::PER_WARP);
-    if (blocks > 8 * sm_count(dev)) blocks = 8 * sm_count(dev);
-    route_kernel<L><<<blocks, 256, 0, st>>>(a);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return (int)e;
-    return launch_plan<void>(p, a, plan_ctas((long long)a.T * a.k), st);
-}
-
-template <typename L>
-int launch_backward(const RouteArgs& a, const float* dw, void* dlogits, int dev, cudaStream_t st) {
-    int blocks = (a.T + 8 * L::PER_WARP - 1) / (8 * L::PER_WARP);
-    if (blocks > 8 * sm_count(dev)) blocks = 8 * sm_count(dev);
-    route_backward_kernel<L><<<blocks, 256, 0, st>>>(a, dw, dlogits);
-    cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? NVFP4_OK : (int)e;
+    const int rc = launch_dependent(route_kernel<L>, token_blocks<L>(a, dev), 256, 0, 0, st, a);
+    return rc ? rc : plan_choices(p, st);
 }
 
 // f(layout) for the element type and the number of experts
@@ -494,20 +542,25 @@ int check_route(int kind, long long ld, int T, int E, int k) {
 
 using namespace nvfp4;
 
+extern "C" long long nvfp4_moe_plan_scratch(int T, int E, int k) {
+    return T > 0 && E > 0 && k > 0 && (long long)T * k > PLAN_CLUSTER_MOST ? 4ll * PLAN_BLOCKS * E : 0;
+}
+
 extern "C" int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* rows, void* slots,
-                              void* source, void* stream) {
+                              void* source, void* scratch, void* stream) {
     if (!experts || !offsets || !tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
     if (T <= 0 || E <= 0 || k <= 0) return NVFP4_ERR_SHAPE;
     if (k > MOE_MAX_CHOICES) return NVFP4_ERR_UNSUPPORTED;
     // (padded rows are counted in 32 bits: up to 127 more for every expert)
     if (E > MOE_MAX_EXPERTS || (long long)T * k + 128ll * E >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
-    const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)rows, (int*)slots, (int*)source, T, E, k};
-    return launch_plan<void>(p, RouteArgs{}, plan_ctas((long long)T * k), (cudaStream_t)stream);
+    if (nvfp4_moe_plan_scratch(T, E, k) && !scratch) return NVFP4_ERR_NULL;
+    const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)rows, (int*)slots, (int*)source, (uint32_t*)scratch, T, E, k};
+    return plan_choices(p, (cudaStream_t)stream);
 }
 
 extern "C" int nvfp4_moe_route(const void* logits, int kind, long long ld, const void* mask, int T, int E, int k, int renormalize,
                                void* weights, void* experts, void* offsets, void* tiles, void* rows, void* slots, void* source,
-                               void* stream) {
+                               void* scratch, void* stream) {
     if (!logits || !weights || !experts || !offsets || !tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
     int rc = check_route(kind, ld, T, E, k);
     if (rc) return rc;
@@ -517,7 +570,8 @@ extern "C" int nvfp4_moe_route(const void* logits, int kind, long long ld, const
     if (err != cudaSuccess) return (int)err;
     const RouteArgs a{logits, ld, (const uint8_t*)mask, (float*)weights, (int*)experts, T, E, k, renormalize,
                       rows_wide(logits, kind, ld)};
-    const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)rows, (int*)slots, (int*)source, T, E, k};
+    if (nvfp4_moe_plan_scratch(T, E, k) && !scratch) return NVFP4_ERR_NULL;
+    const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)rows, (int*)slots, (int*)source, (uint32_t*)scratch, T, E, k};
     return by_kind(kind, E, [&](auto layout) { return launch_route<decltype(layout)>(a, p, dev, (cudaStream_t)stream); });
 }
 
@@ -533,6 +587,8 @@ extern "C" int nvfp4_moe_route_backward(const void* dweights, const void* logits
     const RouteArgs a{logits, ld, nullptr, (float*)const_cast<void*>(weights), (int*)const_cast<void*>(experts), T, E, k, renormalize,
                       rows_wide(logits, kind, ld)};
     return by_kind(kind, E, [&](auto layout) {
-        return launch_backward<decltype(layout)>(a, (const float*)dweights, dlogits, dev, (cudaStream_t)stream);
+        using L = decltype(layout);
+        return launch_dependent(route_backward_kernel<L>, token_blocks<L>(a, dev), 256, 0, 0, (cudaStream_t)stream, a,
+                                (const float*)dweights, dlogits);
     });
 }

@@ -16,6 +16,26 @@ int* status_word(int dev);
 // Budget, in nanoseconds, after which a device-side wait gives up (NVFP4_WAIT_BUDGET_MS, default 2000 ms).
 unsigned long long wait_budget_ns();
 
+// Launches with programmatic dependent launch (and in clusters of `cluster` CTAs where that is not 0): the kernels of a
+// layer are short, and the start of each then hides behind the end of the one before it.
+template <typename... P, typename... A>
+int launch_dependent(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+    return e == cudaSuccess ? NVFP4_OK : (int)e;
+}
+
 // cuTensorMapEncodeTiled through the runtime's driver entry point (the library does not link libcuda).
 // dims / box in elements (innermost first), strides in bytes for dimensions 1..rank-1.
 int encode_tiled(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const void* base, const uint64_t* dims,

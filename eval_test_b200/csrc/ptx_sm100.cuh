@@ -83,6 +83,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_
     }
 }
 
+// Programmatic dependent launch.  A kernel launched with that attribute may start while the kernel before it in the
+// stream still runs: pdl_wait() returns when that kernel has completed and its memory is visible, pdl_launch() says that
+// the next one may start.  Both do nothing in a kernel launched without the attribute.  Every kernel that is launched
+// with it waits before it touches global memory, so the kernels of a stream still take effect in order.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Record the first failure of a launch (device scope; the word may live in mapped host memory).
 __device__ __forceinline__ void report_status(int* status, int code) {
     if (status) atomicCAS_system(status, 0, code);

@@ -36,13 +36,16 @@ class Plan:
     __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "_at")
 
     def __init__(self, num_tokens: int, top_k: int, num_experts: int, device: torch.device):
-        n = num_tokens * top_k
-        size = 2 * (num_experts + 1) + 3 * n
+        n, e = num_tokens * top_k, num_experts + 1
+        # behind the tables: the copies per expert of each block of a large sort
+        size = 2 * e + 3 * n + (_lib.load().nvfp4_moe_plan_scratch(num_tokens, num_experts, top_k) // 4 if n > 4096 else 0)
         # (no copies: nothing is launched, and every expert starts at row 0)
         self.buffer = torch.empty(size, dtype=torch.int32, device=device) if n else torch.zeros(size, dtype=torch.int32, device=device)
         self.num_tokens, self.top_k, self.num_experts = num_tokens, top_k, num_experts
-        base, e, n = self.buffer.data_ptr(), 4 * (num_experts + 1), 4 * n
-        self._at = (base, base + e, base + 2 * e, base + 2 * e + n, base + 2 * e + 2 * n)
+        base = self.buffer.data_ptr()
+        rows = base + 8 * e
+        n *= 4
+        self._at = (base, base + 4 * e, rows, rows + n, rows + 2 * n, rows + 3 * n)
 
     @property
     def device(self) -> torch.device:
@@ -86,7 +89,8 @@ class Plan:
     @property
     def source(self) -> torch.Tensor:
         """[T * k] copy of a row, -1 behind the last."""
-        return self.buffer[2 * (self.num_experts + 1) + 2 * self.num_tokens * self.top_k:]
+        n = self.num_tokens * self.top_k
+        return self.buffer.as_strided((n,), (1,), 2 * (self.num_experts + 1) + 2 * n)
 
 
 class Routing(NamedTuple):

@@ -138,7 +138,8 @@ int nvfp4_quantize_bf16(const void* x, void* packed, void* sf_sw, int rows, int 
  * T tokens choose k of E experts (E <= 1024, k <= 32); copy i = t*k + j is choice j of token t.  The copies
  * are sorted stably by expert into R = T*k rows.  The group sizes stay on the device, so a whole layer can be captured
  * into a graph (eval/nvfp4_grouped_gemm/reference.py:137-201 takes them as a host list).  An expert id outside [0, E)
- * means "not routed": the copy has no row.  No entry point keeps a workspace: what it needs is an argument.
+ * means "not routed": the copy has no row.  No entry point keeps a workspace: what it needs is an argument.  The kernels are launched with programmatic dependent
+ * launch and wait for the kernel before them in the stream before they touch memory.
  * Element types of activations: */
 enum { NVFP4_F32 = 0, NVFP4_F16 = 1, NVFP4_BF16 = 2 };
 
@@ -148,9 +149,11 @@ enum { NVFP4_F32 = 0, NVFP4_F16 = 1, NVFP4_BF16 = 2 };
  *   rows    [T][k] row of a copy, -1: none
  *   slots   [T][k] 128 * tile + row in the tile: where the scales of the copy's row are, -1: none
  *   source  [T*k]  copy of a row, -1 behind the last one
- * all int32.  T, E, k > 0, k <= 32. */
+ * all int32.  T, E, k > 0, k <= 32.  scratch: nvfp4_moe_plan_scratch(T, E, k) bytes (0 for up to 16384 copies: may be
+ * NULL then), 4-byte aligned, not read after the call's kernels. */
 int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* rows, void* slots,
-                   void* source, void* stream);
+                   void* source, void* scratch, void* stream);
+long long nvfp4_moe_plan_scratch(int T, int E, int k);
 
 /* Router: weights [T][k] (fp32) and experts [T][k] (int32) of the k largest of each row of logits [T][E] (element type
  * `kind`, rows `ld` elements apart), largest first, ties to the lowest index, and the plan of that choice.
@@ -159,7 +162,7 @@ int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void
  * experts -1 with weight 0.  k <= E. */
 int nvfp4_moe_route(const void* logits, int kind, long long ld, const void* mask, int T, int E, int k, int renormalize,
                     void* weights, void* experts, void* offsets, void* tiles, void* rows, void* slots, void* source,
-                    void* stream);
+                    void* scratch, void* stream);
 /* Its gradient: dlogits [T][E] (element type `kind`, contiguous) from dweights [T][k] (fp32), with the weights and
  * experts that the router returned; 0 for entries that took no part. */
 int nvfp4_moe_route_backward(const void* dweights, const void* logits, int kind, long long ld, const void* weights,

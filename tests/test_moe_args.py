@@ -5,13 +5,15 @@ import torch
 
 def test_c_entries_reject_bad_arguments(lib):
     P = 32                                                # stands for an aligned pointer; nothing is read
-    plan = (P,) * 5
+    plan = (P,) * 6                                       # five tables and the scratch
     assert lib.nvfp4_moe_plan(None, 4, 4, 2, *plan, None) == -1
     assert lib.nvfp4_moe_plan(P, 0, 4, 2, *plan, None) == -2
     assert lib.nvfp4_moe_plan(P, 4, 0, 2, *plan, None) == -2
     assert lib.nvfp4_moe_plan(P, 4, 1025, 2, *plan, None) == -6
     assert lib.nvfp4_moe_plan(P, 4, 64, 33, *plan, None) == -6
     assert lib.nvfp4_moe_plan(P, 1 << 30, 4, 2, *plan, None) == -6       # copies are counted in 32 bits
+    assert lib.nvfp4_moe_plan_scratch(2048, 64, 8) == 0 and lib.nvfp4_moe_plan_scratch(2049, 64, 8) > 0
+    assert lib.nvfp4_moe_plan(P, 2049, 64, 8, *plan[:5], None, None) == -1
     route = lambda kind=0, ld=8, T=4, E=8, k=2, logits=P: lib.nvfp4_moe_route(  # noqa: E731
         logits, kind, ld, None, T, E, k, 1, P, P, *plan, None)
     assert route(logits=None) == -1

@@ -138,7 +138,8 @@ def test_route_backward_of_rows_without_choices(renormalize):
 
 # ------------------------------------------------------------------------------------------------ plan
 @pytest.mark.parametrize("T,E,k,drop", [(1, 1, 1, 0.0), (1, 64, 8, 0.0), (5, 3, 2, 0.5), (129, 7, 1, 0.0), (1025, 1024, 3, 0.1),
-                                        (3000, 33, 5, 0.3), (20011, 64, 8, 0.0)])
+                                        (3000, 33, 5, 0.3), (20011, 64, 8, 0.0), (5500, 1024, 3, 0.2), (16385, 1, 1, 0.1),
+                                        (4096, 300, 4, 0.0), (70001, 129, 1, 0.0)])
 def test_plan_sorts_stably(T, E, k, drop):
     from eval_test_b200 import moe
     ids = choices(T, E, k, drop, seed=T)
