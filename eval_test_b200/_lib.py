@@ -78,18 +78,18 @@ def load() -> ctypes.CDLL:
     for q in (lib.nvfp4_quantize_f32, lib.nvfp4_quantize_f16, lib.nvfp4_quantize_bf16):
         q.argtypes = [vp, vp, vp, i, i, i, vp]
     ll = ctypes.c_longlong
-    lib.nvfp4_moe_plan.argtypes = [vp, i, i, i, vp, vp, vp, vp, vp, vp, vp]
+    lib.nvfp4_moe_plan.argtypes = [vp, i, i, i] + [vp] * 8
     lib.nvfp4_moe_plan_scratch.argtypes = [i, i, i]
     lib.nvfp4_moe_plan_scratch.restype = ll
-    lib.nvfp4_moe_route.argtypes = [vp, i, ll, vp, i, i, i, i, vp, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.nvfp4_moe_route.argtypes = [vp, i, ll, vp, i, i, i, i] + [vp] * 10
     lib.nvfp4_moe_route_backward.argtypes = [vp, vp, i, ll, vp, vp, i, i, i, i, vp, vp]
     lib.nvfp4_moe_dispatch.argtypes = [vp, i, ll, vp, vp, i, i, i, i, vp, vp]
     lib.nvfp4_moe_combine.argtypes = [vp, i, ll, vp, vp, i, i, i, vp, i, vp]
     lib.nvfp4_moe_combine_backward.argtypes = [vp, i, ll, vp, i, ll, vp, vp, vp, i, i, i, i, vp, vp, vp]
     lib.nvfp4_moe_dispatch_nvfp4.argtypes = [vp, i, ll, vp, vp, vp, i, i, i, i, vp, vp, vp]
-    lib.nvfp4_moe_gemm.argtypes = [vp] * 8 + [i, i, i, i, f, vp]
-    lib.nvfp4_moe_dual_gemm.argtypes = [vp] * 10 + [i, i, i, i, f, vp]
-    lib.nvfp4_moe_dual_gemm_nvfp4.argtypes = [vp] * 11 + [i, i, i, i, f, vp]
+    lib.nvfp4_moe_gemm.argtypes = [vp] * 9 + [i, i, i, i, f, vp]
+    lib.nvfp4_moe_dual_gemm.argtypes = [vp] * 11 + [i, i, i, i, f, vp]
+    lib.nvfp4_moe_dual_gemm_nvfp4.argtypes = [vp] * 12 + [i, i, i, i, f, vp]
     lib.nvfp4_device_status.argtypes = [i, i]
     lib.nvfp4_wait_selftest.argtypes = [i, ctypes.POINTER(ctypes.c_double), vp]
     lib.nvfp4_strerror.argtypes = [i]

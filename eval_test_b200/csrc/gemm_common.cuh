@@ -62,11 +62,8 @@ struct GatherOut {
 // parameter of the gathering instantiations only.
 struct GatherMaps { CUtensorMap m[8]; };
 struct NoGatherMaps { int unused; };
-// Expert products: the same operand A as `tmap_a` in boxes of 16 rows, for tiles with few rows.
-struct ExpertMaps { CUtensorMap a16; };
-template <bool GATHER, bool EXPERTS = false> struct GatherMapsOf { using type = NoGatherMaps; };
-template <> struct GatherMapsOf<true, false> { using type = GatherMaps; };
-template <> struct GatherMapsOf<false, true> { using type = ExpertMaps; };
+template <bool GATHER> struct GatherMapsOf { using type = NoGatherMaps; };
+template <> struct GatherMapsOf<true> { using type = GatherMaps; };
 
 // What one epilogue warp needs for a gathering store: the maps, GATHER_BOXES x 4 KB of shared memory of its own (1024-byte
 // aligned; a box of 32 rows x 128 bytes each, filled in turn) and where its rows are in the full C.
@@ -87,17 +84,6 @@ struct GatherCtx {
     int cc;                // chunk of the tile being stored
 };
 
-// Products of tokens sorted by expert: A and C are [M][...] rows in expert order, B holds every expert's weights ([E][N]
-// [K/2]), and the sizes of the groups are on the device only (made by nvfp4_moe_plan).  An expert's rows start
-// anywhere in A (a TMA box may start at any row; what it reads of the next expert's rows is not stored); its scale atoms
-// follow the 128-row tiles, which are counted per expert.
-struct ExpertGroups {
-    const int* offsets = nullptr;   // [E+1] first row of each expert
-    const int* tiles = nullptr;     // [E+1] first 128-row tile of each expert
-    const float* alpha = nullptr;   // [E] factors on top of the launch's alpha, or null
-    int E = 0;
-};
-
 struct GemmParams {
     const uint8_t* sfa;   // swizzled scales of A  [L][ceil(M/128)][K/64][512]
     const uint8_t* sfb;   // swizzled scales of B (B1 for the dual GEMM)
@@ -106,7 +92,6 @@ struct GemmParams {
     uint8_t* cq = nullptr;   // NVFP4 output instead of fp16: packed e2m1 [L][M][N/2] ...
     uint8_t* sfc = nullptr;  // ... and its block scales, swizzled [L][ceil(M/128)][N/64][512]
     GatherOut gather;
-    ExpertGroups experts;
     int M, N, K, L;
     float alpha;
     int* status;
@@ -140,9 +125,6 @@ struct TileInfo {
     __half* c;                // output of this problem / batch
     size_t sf_row_block;      // bytes of one 128-row scale block = K/64 * 512
     int M, N, kiters, l, m0, n0, nb_valid;
-    int lb;                   // batch of the B operand
-    int row_tile;             // 128-row tile among all scale tiles of A
-    float alpha;
 };
 
 // Tile order: bands of 16 row-tiles; inside a band the row-tile index runs fastest, so the CTAs that
@@ -168,35 +150,12 @@ __device__ __forceinline__ float silu_mul(float x, float y) { return __fdividef(
 
 // Tile t of a plain / dual GEMM (all batches share the maps; the batch is the third TMA coordinate) or of a
 // grouped GEMM (binary search of the group whose tile range holds t; column tile fastest inside a group).
-// EXPERTS: binary search of the expert whose row tiles hold the tile's (empty experts have none), column tile fastest.
-template <int BN, bool DUAL, bool GROUPED, bool EXPERTS = false>
+template <int BN, bool DUAL, bool GROUPED>
 __device__ __forceinline__ TileInfo locate(int t, const GemmParams& p, const CUtensorMap* ta, const CUtensorMap* tb,
                                            const CUtensorMap* tb2) {
     constexpr int NB_BLOCKS = (DUAL ? 2 * BN : BN) / 128;
     TileInfo ti;
-    ti.alpha = p.alpha;
-    if (EXPERTS) {
-        const int tiles_n = p.N / BN;
-        const int u = t / tiles_n, nt = t - u * tiles_n;
-        int lo = 0, hi = p.experts.E - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (__ldg(p.experts.tiles + mid) <= u) lo = mid; else hi = mid - 1;
-        }
-        ti.ta = ta; ti.tb = tb; ti.tb2 = tb2;
-        ti.m0 = __ldg(p.experts.offsets + lo) + (u - __ldg(p.experts.tiles + lo)) * BM;
-        ti.M = __ldg(p.experts.offsets + lo + 1);
-        ti.N = p.N; ti.kiters = p.K / BK;
-        ti.sf_row_block = (size_t)(p.K / 64) * 512;
-        ti.l = 0; ti.lb = lo; ti.row_tile = u; ti.n0 = nt * BN;
-        ti.sfa_t = p.sfa + (size_t)u * ti.sf_row_block;
-        const size_t blk = (size_t)lo * (p.N / 128) + ti.n0 / 128;
-        ti.sfb_t = p.sfb + blk * ti.sf_row_block;
-        ti.sfb2_t = DUAL ? p.sfb2 + blk * ti.sf_row_block : nullptr;
-        ti.c = p.c;
-        ti.nb_valid = NB_BLOCKS;
-        if (p.experts.alpha) ti.alpha *= __ldg(p.experts.alpha + lo);
-    } else if (GROUPED) {
+    if (GROUPED) {
         int lo = 0, hi = p.G - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -216,7 +175,7 @@ __device__ __forceinline__ TileInfo locate(int t, const GemmParams& p, const CUt
         const int K = __ldg(&e->K);
         ti.kiters = K / BK;
         ti.sf_row_block = (size_t)(K / 64) * 512;
-        ti.l = ti.lb = 0; ti.row_tile = mt; ti.m0 = mt * BM; ti.n0 = nt * BN;
+        ti.l = 0; ti.m0 = mt * BM; ti.n0 = nt * BN;
         ti.sfa_t = e->sfa + (size_t)mt * ti.sf_row_block;
         ti.sfb_t = e->sfb + (size_t)(ti.n0 / 128) * ti.sf_row_block;
         ti.sfb2_t = nullptr;
@@ -229,8 +188,8 @@ __device__ __forceinline__ TileInfo locate(int t, const GemmParams& p, const CUt
         ti.ta = ta; ti.tb = tb; ti.tb2 = tb2;
         ti.M = p.M; ti.N = p.N; ti.kiters = p.K / BK;
         ti.sf_row_block = (size_t)(p.K / 64) * 512;
-        ti.l = ti.lb = tc.l; ti.row_tile = tc.l * tiles_m + tc.mt; ti.m0 = tc.mt * BM; ti.n0 = tc.nt * BN;
-        ti.sfa_t = p.sfa + (size_t)ti.row_tile * ti.sf_row_block;
+        ti.l = tc.l; ti.m0 = tc.mt * BM; ti.n0 = tc.nt * BN;
+        ti.sfa_t = p.sfa + ((size_t)tc.l * tiles_m + tc.mt) * ti.sf_row_block;
         const size_t blk = (size_t)tc.l * RB + ti.n0 / 128;
         ti.sfb_t = p.sfb + blk * ti.sf_row_block;
         ti.sfb2_t = DUAL ? p.sfb2 + blk * ti.sf_row_block : nullptr;

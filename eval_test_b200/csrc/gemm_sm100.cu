@@ -39,12 +39,11 @@ namespace nvfp4 {
 // BN: output columns per tile (GEMM: 128 or 256; DUAL: 128, the MMA is 256 wide over [B1;B2]).
 // QOUT: the epilogue writes NVFP4 (packed codes + swizzled block scales) instead of fp16.
 // GATHER: the fp16 output goes to the full C buffer of every rank of an N-sharded run (fused all-gather).
-// EXPERTS: rows sorted by expert, group sizes on the device (ExpertGroups).
-template <int BN, bool DUAL, bool GROUPED, int STAGES, bool QOUT = false, bool GATHER = false, bool EXPERTS = false>
+template <int BN, bool DUAL, bool GROUPED, int STAGES, bool QOUT = false, bool GATHER = false>
 __global__ void __launch_bounds__(GEMM_THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
             const __grid_constant__ CUtensorMap tmap_b2,
-            const __grid_constant__ typename GatherMapsOf<GATHER, EXPERTS>::type gmaps, const GemmParams p) {
+            const __grid_constant__ typename GatherMapsOf<GATHER>::type gmaps, const GemmParams p) {
     constexpr int MMA_N = DUAL ? 2 * BN : BN;          // rows of the B tile in shared memory
     constexpr int NB_BLOCKS = MMA_N / 128;             // 128-row scale blocks of B per stage
     constexpr uint32_t A_BYTES = BM * 128;
@@ -113,12 +112,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
         tmem_base = tmem_base_slot;
     }
 
-    if (EXPERTS) {
-        pdl_wait();
-        pdl_launch();
-    }
-    // (experts: the tile count comes from the plan; a launch has enough CTAs for the most there can be)
-    const int total_tiles = EXPERTS ? __ldg(p.experts.tiles + p.experts.E) * (p.N / BN) : p.total_tiles;
+    const int total_tiles = p.total_tiles;
 
     if (warp == 0) {
         // ------------------------------------------------------------------ TMA producer (one lane)
@@ -129,7 +123,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
             long long prof_empty = 0;
 #endif
             for (int t = blockIdx.x; alive && t < total_tiles; t += gridDim.x) {
-                const TileInfo ti = locate<BN, DUAL, GROUPED, EXPERTS>(t, p, &tmap_a, &tmap_b, &tmap_b2);
+                const TileInfo ti = locate<BN, DUAL, GROUPED>(t, p, &tmap_a, &tmap_b, &tmap_b2);
                 for (int kit = 0; kit < ti.kiters; kit++, it++) {
                     const int slot = it % STAGES;
                     bool free_;
@@ -152,19 +146,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
                     const uint32_t sSFA = sB + B_BYTES;
                     const uint32_t sSFB = sSFA + SFA_BYTES;
                     const int k0 = kit * BK;
-                    // experts with up to 64 rows in the tile: boxes of 16 rows.  What the rest of the A tile holds
-                    // then belongs to an earlier tile; every accumulator row is a product of its own row of A
-                    const int boxes = EXPERTS && ti.M - ti.m0 <= 64 ? (ti.M - ti.m0 + 15) / 16 : 0;
-                    const uint32_t a_bytes = boxes ? (uint32_t)boxes * 2048u : A_BYTES;
-                    const uint32_t tx = a_bytes + B_BYTES + SFA_BYTES + (uint32_t)ti.nb_valid * 2048u;
+                    const uint32_t tx = A_BYTES + B_BYTES + SFA_BYTES + (uint32_t)ti.nb_valid * 2048u;
                     mbar_arrive_expect_tx(full, tx);
-                    if constexpr (EXPERTS) {
-                        for (int j = 0; j < boxes; j++)
-                            tma_load_3d(sA + j * 2048u, &gmaps.a16, k0, ti.m0 + 16 * j, 0, full);
-                    }
-                    if (!boxes) tma_load_3d(sA, ti.ta, k0, ti.m0, ti.l, full);
-                    tma_load_3d(sB, ti.tb, k0, ti.n0, ti.lb, full);
-                    if (DUAL) tma_load_3d(sB + BN * 128, ti.tb2, k0, ti.n0, ti.lb, full);
+                    tma_load_3d(sA, ti.ta, k0, ti.m0, ti.l, full);
+                    tma_load_3d(sB, ti.tb, k0, ti.n0, ti.l, full);
+                    if (DUAL) tma_load_3d(sB + BN * 128, ti.tb2, k0, ti.n0, ti.l, full);
                     const size_t koff = (size_t)(k0 / 64) * 512;
                     bulk_g2s(sSFA, ti.sfa_t + koff, 2048u, full);
                     if (DUAL) {
@@ -207,7 +193,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
                 }
                 tc_fence_after_sync();
                 const uint32_t t_acc = tmem_base + buf * ACC1_OFF;
-                const int kiters = locate<BN, DUAL, GROUPED, EXPERTS>(t, p, &tmap_a, &tmap_b, &tmap_b2).kiters;
+                const int kiters = locate<BN, DUAL, GROUPED>(t, p, &tmap_a, &tmap_b, &tmap_b2).kiters;
                 for (int kit = 0; kit < kiters; kit++, it++) {
                     const int slot = it % STAGES;
                     bool got;
@@ -277,18 +263,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
             gc.stage = reinterpret_cast<uint4*>(smem_raw + (gc.stage_smem - smem_u32(smem_raw)));
             gc.uses = 0;
         }
-        if constexpr (EXPERTS) {
-            // rows behind the last copy (choices that were dropped): zero, so that sums over the buffer are sums over copies
-            const size_t row_bytes = QOUT ? (size_t)p.N / 2 : (size_t)p.N * 2;
-            uint8_t* out = QOUT ? p.cq : reinterpret_cast<uint8_t*>(p.c);
-            const uint32_t zero[8] = {};
-            const size_t end = (size_t)p.M * row_bytes / 32;
-            for (size_t i = (size_t)__ldg(p.experts.offsets + p.experts.E) * row_bytes / 32 + (size_t)blockIdx.x * 128 + threadIdx.x - 64;
-                 i < end; i += (size_t)gridDim.x * 128)
-                st_global_256(out + i * 32, zero);
-        }
         for (int t = blockIdx.x; t < total_tiles; t += gridDim.x, tile_it++) {
-            const TileInfo ti = locate<BN, DUAL, GROUPED, EXPERTS>(t, p, &tmap_a, &tmap_b, &tmap_b2);
+            const TileInfo ti = locate<BN, DUAL, GROUPED>(t, p, &tmap_a, &tmap_b, &tmap_b2);
             const int row = ti.m0 + q * 32 + lane;
             const int n0 = ti.n0;
             const uint32_t buf = tile_it & 1;
@@ -311,16 +287,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ 
             if (QOUT) {
                 const size_t grow = (size_t)ti.l * ti.M + srow;                       // row of the [L*M][N] output
                 qo.codes = p.cq + grow * (size_t)(ti.N / 2) + n0 / 2;
-                const int in_tile = EXPERTS ? q * 32 + lane : srow % 128;
-                const size_t rb = EXPERTS ? (size_t)ti.row_tile : (size_t)ti.l * ((ti.M + 127) / 128) + srow / 128;   // 128-row block of the scales
-                qo.scales = p.sfc + (rb * (size_t)(ti.N / 64) + n0 / 64) * 512 + (in_tile % 32) * 16 + (in_tile / 32) * 4;
+                const size_t rb = (size_t)ti.l * ((ti.M + 127) / 128) + srow / 128;   // 128-row block of the scales
+                qo.scales = p.sfc + (rb * (size_t)(ti.N / 64) + n0 / 64) * 512 + (srow % 32) * 16 + ((srow % 128) / 32) * 4;
             }
             // buffer 0 shares its last OVERLAP columns, buffer 1 its first
             if (buf == 0)
                 epilogue_tile<BN, DUAL, int(ACC1_OFF) / 32, OV_CHUNKS, false, QOUT, GATHER>(
-                    t_lane, crow, row < ti.M, n0, ti.N, EXPERTS ? ti.alpha : p.alpha, ovl_free, lane, &qo, &gc);
+                    t_lane, crow, row < ti.M, n0, ti.N, p.alpha, ovl_free, lane, &qo, &gc);
             else
-                epilogue_tile<BN, DUAL, 0, OV_CHUNKS, false, QOUT, GATHER>(t_lane, crow, row < ti.M, n0, ti.N, EXPERTS ? ti.alpha : p.alpha,
+                epilogue_tile<BN, DUAL, 0, OV_CHUNKS, false, QOUT, GATHER>(t_lane, crow, row < ti.M, n0, ti.N, p.alpha,
                                                                           ovl_free, lane, &qo, &gc);
             tc_fence_before_sync();
             __syncwarp();
@@ -382,15 +357,15 @@ int make_scale_tmap(CUtensorMap* map, const void* base, long atoms) {
     return NVFP4_OK;
 }
 
-template <int BN, bool DUAL, bool GROUPED, int STAGES, bool QOUT = false, bool GATHER = false, bool EXPERTS = false>
+template <int BN, bool DUAL, bool GROUPED, int STAGES, bool QOUT = false, bool GATHER = false>
 static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, const GemmParams& p,
-                       cudaStream_t stream, const typename GatherMapsOf<GATHER, EXPERTS>::type& gm = {}) {
+                       cudaStream_t stream, const typename GatherMapsOf<GATHER>::type& gm = {}) {
     constexpr int MMA_N = DUAL ? 2 * BN : BN;
     constexpr size_t STAGE = 128 * 128 + MMA_N * 128 + 2048 + (MMA_N / 128) * 2048;
     // + slack for the 1024-byte alignment (+ the 4 KB boxes of the epilogue warps for the gathering stores)
     constexpr size_t SMEM = STAGES * STAGE + 1024 + (GATHER ? 4 * GATHER_BOXES * 4096 : 0);
     static_assert(SMEM <= 227 * 1024 - 256, "shared memory");
-    auto kern = gemm_kernel<BN, DUAL, GROUPED, STAGES, QOUT, GATHER, EXPERTS>;
+    auto kern = gemm_kernel<BN, DUAL, GROUPED, STAGES, QOUT, GATHER>;
     static bool configured[64] = {};
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -403,13 +378,9 @@ static int launch_gemm(const CUtensorMap& ta, const CUtensorMap& tb, const CUten
     }
     if (p.total_tiles <= 0) return NVFP4_OK;
     const int grid = p.total_tiles < sm_count(dev) ? p.total_tiles : sm_count(dev);
-    if constexpr (EXPERTS) {
-        return launch_dependent(kern, grid, GEMM_THREADS, SMEM, 0, stream, ta, tb, tb2, gm, p);
-    } else {
-        kern<<<grid, GEMM_THREADS, SMEM, stream>>>(ta, tb, tb2, gm, p);
-        e = cudaGetLastError();
-        return e == cudaSuccess ? NVFP4_OK : (int)e;
-    }
+    kern<<<grid, GEMM_THREADS, SMEM, stream>>>(ta, tb, tb2, gm, p);
+    e = cudaGetLastError();
+    return e == cudaSuccess ? NVFP4_OK : (int)e;
 }
 
 static int check_common(const void* const* ptrs, int nptr, int M, int N, int K, int L) {
@@ -650,70 +621,6 @@ extern "C" int nvfp4_dual_gemm_allgather(const void* a, const void* b1, const vo
     p.table = nullptr; p.G = 0;
     p.total_tiles = ((M + BM - 1) / BM) * (N_local / 128) * L;
     return launch_gemm<128, true, false, 3, false, true>(ta, tb1, tb2, p, (cudaStream_t)stream, gm);
-}
-
-// ------------------------------------------------------------------------------------------ products of sorted tokens
-// Row tiles that R copies over E experts can fill at most: every expert that has rows has at most one tile that is not
-// full.
-static long most_row_tiles(int R, int E) {
-    const int active = R < E ? R : E;
-    return active + (long)(R - active) / 128;
-}
-
-// What the three entry points share.  dual: b2 / sfb2 are used; q: the output is packed codes (c) and scales (sfc).
-static int expert_product(bool dual, bool q, const void* a, const void* sfa_sw, const void* b, const void* sfb_sw, const void* b2,
-                          const void* sfb2_sw, const void* offsets, const void* tiles, const void* alphas, void* c, void* sfc,
-                          int R, int E, int N, int K, float alpha, void* stream) {
-    const void* ptrs[9] = {a, sfa_sw, b, sfb_sw, dual ? b2 : b, dual ? sfb2_sw : sfb_sw, q ? sfc : c, c, c};
-    int rc = check_common(ptrs, 9, R, N, K, E);
-    if (rc) return rc;
-    if (!offsets || !tiles) return NVFP4_ERR_NULL;
-    if (((uintptr_t)offsets | (uintptr_t)tiles | (uintptr_t)alphas) & 3) return NVFP4_ERR_ALIGN;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
-    const long row_tiles = most_row_tiles(R, E);
-    if (row_tiles * (N / 128) >= (1l << 31)) return NVFP4_ERR_UNSUPPORTED;
-    // 256-wide tiles when N allows and they still fill the machine, else 128-wide, as for the grouped GEMM
-    const bool wide = !dual && N % 256 == 0 && row_tiles * (N / 256) >= sm_count(dev);
-    CUtensorMap ta, tb, tb2;
-    ExpertMaps em;
-    if ((rc = make_operand_tmap(&ta, a, R, K, 1, 128)) || (rc = make_operand_tmap(&em.a16, a, R, K, 1, 16)) ||
-        (rc = make_operand_tmap(&tb, b, N, K, E, wide ? 256 : 128)))
-        return rc;
-    tb2 = tb;
-    if (dual && (rc = make_operand_tmap(&tb2, b2, N, K, E, 128))) return rc;
-    GemmParams p;
-    p.sfa = (const uint8_t*)sfa_sw; p.sfb = (const uint8_t*)sfb_sw; p.sfb2 = (const uint8_t*)sfb2_sw;
-    p.c = q ? nullptr : (__half*)c;
-    if (q) { p.cq = (uint8_t*)c; p.sfc = (uint8_t*)sfc; }
-    p.experts.offsets = (const int*)offsets; p.experts.tiles = (const int*)tiles; p.experts.alpha = (const float*)alphas;
-    p.experts.E = E;
-    p.M = R; p.N = N; p.K = K; p.L = 1; p.alpha = alpha;
-    p.status = status_word(dev);
-    p.budget_ns = wait_budget_ns();
-    p.table = nullptr; p.G = 0;
-    p.total_tiles = (int)(row_tiles * (N / (wide ? 256 : 128)));
-    cudaStream_t st = (cudaStream_t)stream;
-    if (dual && q) return launch_gemm<128, true, false, 4, true, false, true>(ta, tb, tb2, p, st, em);
-    if (dual) return launch_gemm<128, true, false, 4, false, false, true>(ta, tb, tb2, p, st, em);
-    if (wide) return launch_gemm<256, false, false, 4, false, false, true>(ta, tb, tb2, p, st, em);
-    return launch_gemm<128, false, false, 6, false, false, true>(ta, tb, tb2, p, st, em);
-}
-
-extern "C" int nvfp4_moe_gemm(const void* a, const void* sfa_sw, const void* b, const void* sfb_sw, const void* offsets,
-                              const void* tiles, const void* alphas, void* c, int R, int E, int N, int K, float alpha, void* stream) {
-    return expert_product(false, false, a, sfa_sw, b, sfb_sw, nullptr, nullptr, offsets, tiles, alphas, c, nullptr, R, E, N, K, alpha, stream);
-}
-extern "C" int nvfp4_moe_dual_gemm(const void* a, const void* sfa_sw, const void* b1, const void* sfb1_sw, const void* b2,
-                                   const void* sfb2_sw, const void* offsets, const void* tiles, const void* alphas, void* c, int R,
-                                   int E, int N, int K, float alpha, void* stream) {
-    return expert_product(true, false, a, sfa_sw, b1, sfb1_sw, b2, sfb2_sw, offsets, tiles, alphas, c, nullptr, R, E, N, K, alpha, stream);
-}
-extern "C" int nvfp4_moe_dual_gemm_nvfp4(const void* a, const void* sfa_sw, const void* b1, const void* sfb1_sw, const void* b2,
-                                         const void* sfb2_sw, const void* offsets, const void* tiles, const void* alphas,
-                                         void* c_packed, void* sfc_sw, int R, int E, int N, int K, float alpha, void* stream) {
-    return expert_product(true, true, a, sfa_sw, b1, sfb1_sw, b2, sfb2_sw, offsets, tiles, alphas, c_packed, sfc_sw, R, E, N, K, alpha, stream);
 }
 
 // ------------------------------------------------------------------------------------------ grouped GEMM

@@ -261,6 +261,7 @@ struct PlanArgs {
     const int* experts;        // [T][k]
     int* offsets;              // [E+1] first sorted row of each expert
     int* tiles;                // [E+1] first 128-row tile of each expert
+    int* wide;                 // [E+1] first 256-row tile of each expert
     int* rows;                 // [T][k] sorted row of a copy, -1: none
     int* slots;                // [T][k] the row counted with every expert padded to whole tiles, -1: none
     int* source;               // [T*k] copy of a sorted row, -1 behind the last
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_count_kernel(const PlanA
 //     scratch; L: the warps choose their tokens' experts first, in that layout (few tokens: router and plan in one);
 //   spread: PLAN_BLOCKS blocks on as many SMs, whose counts plan_count_kernel has left in memory.
 // 131072 copies, 64 experts: 25.8 us in a cluster of 8 (what bounds it is the scattered stores and the votes of eight
-// SMs), SPREAD_MEASURED us spread over 128 blocks, the counting included; up to 16384 copies the one launch is faster.
+// SMs), 13 us spread over 128 blocks, the counting included; up to 16384 copies the one launch is faster.
 template <typename L, bool SPREAD>
 __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs p, const RouteArgs a) {
     extern __shared__ uint32_t plan_smem[];
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     uint32_t* total = hist + PLAN_WARPS * p.E;          // [E] copies of this block; spread: of all blocks
     uint32_t* base = total + p.E;                       // [E] first row of this block's copies
     int* shift = reinterpret_cast<int*>(base + p.E);    // [E] slot - row of the expert
-    __shared__ uint32_t warp_total[2][PLAN_WARPS];
+    __shared__ uint32_t warp_total[3][PLAN_WARPS];
     __shared__ uint32_t live_rows;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = SPREAD ? blockIdx.x : cluster_ctarank(), ctas = SPREAD ? gridDim.x : cluster_size();
@@ -415,24 +416,27 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
             }
         }
     }
-    const uint32_t ntiles = (count + 127) / 128;
-    uint32_t rows_to = count, tiles_to = ntiles;        // inclusive sums over the warp's experts
+    const uint32_t ntiles = (count + 127) / 128, nwide = (count + 255) / 256;
+    uint32_t rows_to = count, tiles_to = ntiles, wide_to = nwide;    // inclusive sums over the warp's experts
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, rows_to, o), y = __shfl_up_sync(0xffffffffu, tiles_to, o);
-        if (lane >= o) { rows_to += x; tiles_to += y; }
+        const uint32_t x = __shfl_up_sync(0xffffffffu, rows_to, o), y = __shfl_up_sync(0xffffffffu, tiles_to, o),
+                       z = __shfl_up_sync(0xffffffffu, wide_to, o);
+        if (lane >= o) { rows_to += x; tiles_to += y; wide_to += z; }
     }
-    if (lane == 31) { warp_total[0][warp] = rows_to; warp_total[1][warp] = tiles_to; }
+    if (lane == 31) { warp_total[0][warp] = rows_to; warp_total[1][warp] = tiles_to; warp_total[2][warp] = wide_to; }
     __syncthreads();
-    uint32_t row0 = rows_to - count, tile0 = tiles_to - ntiles;
-    for (int w = 0; w < warp; w++) { row0 += warp_total[0][w]; tile0 += warp_total[1][w]; }
+    uint32_t row0 = rows_to - count, tile0 = tiles_to - ntiles, wide0 = wide_to - nwide;
+    for (int w = 0; w < warp; w++) { row0 += warp_total[0][w]; tile0 += warp_total[1][w]; wide0 += warp_total[2][w]; }
     if (threadIdx.x < p.E) {
         base[threadIdx.x] = row0 + before;
         shift[threadIdx.x] = (int)(tile0 * 128u) - (int)row0;
-        if (rank == 0) { p.offsets[threadIdx.x] = (int)row0; p.tiles[threadIdx.x] = (int)tile0; }
+        if (rank == 0) { p.offsets[threadIdx.x] = (int)row0; p.tiles[threadIdx.x] = (int)tile0; p.wide[threadIdx.x] = (int)wide0; }
         if (threadIdx.x == p.E - 1) {
             live_rows = row0 + count;
-            if (rank == 0) { p.offsets[p.E] = (int)(row0 + count); p.tiles[p.E] = (int)(tile0 + ntiles); }
+            if (rank == 0) {
+                p.offsets[p.E] = (int)(row0 + count); p.tiles[p.E] = (int)(tile0 + ntiles); p.wide[p.E] = (int)(wide0 + nwide);
+            }
         }
     }
     // also: no CTA of a cluster leaves while a peer may still read its counts
@@ -546,22 +550,22 @@ extern "C" long long nvfp4_moe_plan_scratch(int T, int E, int k) {
     return T > 0 && E > 0 && k > 0 && (long long)T * k > PLAN_CLUSTER_MOST ? 4ll * PLAN_BLOCKS * E : 0;
 }
 
-extern "C" int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* rows, void* slots,
-                              void* source, void* scratch, void* stream) {
-    if (!experts || !offsets || !tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
+extern "C" int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* wide_tiles, void* rows,
+                              void* slots, void* source, void* scratch, void* stream) {
+    if (!experts || !offsets || !tiles || !wide_tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
     if (T <= 0 || E <= 0 || k <= 0) return NVFP4_ERR_SHAPE;
     if (k > MOE_MAX_CHOICES) return NVFP4_ERR_UNSUPPORTED;
     // (padded rows are counted in 32 bits: up to 127 more for every expert)
     if (E > MOE_MAX_EXPERTS || (long long)T * k + 128ll * E >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
     if (nvfp4_moe_plan_scratch(T, E, k) && !scratch) return NVFP4_ERR_NULL;
-    const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)rows, (int*)slots, (int*)source, (uint32_t*)scratch, T, E, k};
+    const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)wide_tiles, (int*)rows, (int*)slots, (int*)source, (uint32_t*)scratch, T, E, k};
     return plan_choices(p, (cudaStream_t)stream);
 }
 
 extern "C" int nvfp4_moe_route(const void* logits, int kind, long long ld, const void* mask, int T, int E, int k, int renormalize,
-                               void* weights, void* experts, void* offsets, void* tiles, void* rows, void* slots, void* source,
-                               void* scratch, void* stream) {
-    if (!logits || !weights || !experts || !offsets || !tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
+                               void* weights, void* experts, void* offsets, void* tiles, void* wide_tiles, void* rows, void* slots,
+                               void* source, void* scratch, void* stream) {
+    if (!logits || !weights || !experts || !offsets || !tiles || !wide_tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
     int rc = check_route(kind, ld, T, E, k);
     if (rc) return rc;
     if ((long long)T * k + 128ll * E >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
@@ -571,7 +575,7 @@ extern "C" int nvfp4_moe_route(const void* logits, int kind, long long ld, const
     const RouteArgs a{logits, ld, (const uint8_t*)mask, (float*)weights, (int*)experts, T, E, k, renormalize,
                       rows_wide(logits, kind, ld)};
     if (nvfp4_moe_plan_scratch(T, E, k) && !scratch) return NVFP4_ERR_NULL;
-    const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)rows, (int*)slots, (int*)source, (uint32_t*)scratch, T, E, k};
+    const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)wide_tiles, (int*)rows, (int*)slots, (int*)source, (uint32_t*)scratch, T, E, k};
     return by_kind(kind, E, [&](auto layout) { return launch_route<decltype(layout)>(a, p, dev, (cudaStream_t)stream); });
 }
 

@@ -31,21 +31,21 @@ _KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
 class Plan:
-    """How the copies of a batch are sorted (``nvfp4_moe_plan``).  One int32 buffer on the batch's device holds its five
+    """How the copies of a batch are sorted (``nvfp4_moe_plan``).  One int32 buffer on the batch's device holds its six
     tables; the views are made when they are asked for (a call of the layer needs only their addresses)."""
     __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "_at")
 
     def __init__(self, num_tokens: int, top_k: int, num_experts: int, device: torch.device):
         n, e = num_tokens * top_k, num_experts + 1
         # behind the tables: the copies per expert of each block of a large sort
-        size = 2 * e + 3 * n + (_lib.load().nvfp4_moe_plan_scratch(num_tokens, num_experts, top_k) // 4 if n > 4096 else 0)
+        size = 3 * e + 3 * n + (_lib.load().nvfp4_moe_plan_scratch(num_tokens, num_experts, top_k) // 4 if n > 4096 else 0)
         # (no copies: nothing is launched, and every expert starts at row 0)
         self.buffer = torch.empty(size, dtype=torch.int32, device=device) if n else torch.zeros(size, dtype=torch.int32, device=device)
         self.num_tokens, self.top_k, self.num_experts = num_tokens, top_k, num_experts
         base = self.buffer.data_ptr()
-        rows = base + 8 * e
+        rows = base + 12 * e
         n *= 4
-        self._at = (base, base + 4 * e, rows, rows + n, rows + 2 * n, rows + 3 * n)
+        self._at = (base, base + 4 * e, base + 8 * e, rows, rows + n, rows + 2 * n, rows + 3 * n)
 
     @property
     def device(self) -> torch.device:
@@ -62,35 +62,42 @@ class Plan:
         active = min(copies, self.num_experts)
         return active + (copies - active) // 128
 
+    def _per_expert(self, i: int) -> torch.Tensor:
+        e = self.num_experts + 1
+        return self.buffer.as_strided((e,), (1,), i * e)
+
+    def _per_copy(self, i: int, shape, strides) -> torch.Tensor:
+        return self.buffer.as_strided(shape, strides, 3 * (self.num_experts + 1) + i * self.num_tokens * self.top_k)
+
     @property
     def offsets(self) -> torch.Tensor:
         """[E + 1] first row of each expert; offsets[E] rows are in use."""
-        return self.buffer[:self.num_experts + 1]
+        return self._per_expert(0)
 
     @property
     def tiles(self) -> torch.Tensor:
         """[E + 1] first 128-row tile of each expert."""
-        return self.buffer[self.num_experts + 1:2 * (self.num_experts + 1)]
+        return self._per_expert(1)
 
-    def _table(self, i: int) -> torch.Tensor:
-        return self.buffer.as_strided((self.num_tokens, self.top_k), (self.top_k, 1),
-                                      2 * (self.num_experts + 1) + i * self.num_tokens * self.top_k)
+    @property
+    def wide_tiles(self) -> torch.Tensor:
+        """[E + 1] first 256-row tile of each expert."""
+        return self._per_expert(2)
 
     @property
     def rows(self) -> torch.Tensor:
         """[T, k] row of a copy, -1: not routed."""
-        return self._table(0)
+        return self._per_copy(0, (self.num_tokens, self.top_k), (self.top_k, 1))
 
     @property
     def slots(self) -> torch.Tensor:
-        """[T, k] row counted with every expert padded to whole tiles, -1: not routed."""
-        return self._table(1)
+        """[T, k] row counted with every expert padded to whole 128-row tiles, -1: not routed."""
+        return self._per_copy(1, (self.num_tokens, self.top_k), (self.top_k, 1))
 
     @property
     def source(self) -> torch.Tensor:
         """[T * k] copy of a row, -1 behind the last."""
-        n = self.num_tokens * self.top_k
-        return self.buffer.as_strided((n,), (1,), 2 * (self.num_experts + 1) + 2 * n)
+        return self._per_copy(2, (self.num_tokens * self.top_k,), (1,))
 
 
 class Routing(NamedTuple):
@@ -216,7 +223,7 @@ def dispatch(x: torch.Tensor, plan: Plan) -> torch.Tensor:
     _same_device(x.device, plan)
     out = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
     if out.numel():
-        _call("nvfp4_moe_dispatch", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[2], plan._at[0], T,
+        _call("nvfp4_moe_dispatch", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[3], plan._at[0], T,
               plan.num_experts, k, H, out.data_ptr())
     return out
 
@@ -242,7 +249,7 @@ def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dt
     out = make((T, H), dtype=dtype, device=y.device)
     if out.numel() and k:
         _call("nvfp4_moe_combine", y.device, y.data_ptr(), _KINDS[y.dtype], ld, None if weights is None else weights.data_ptr(),
-              plan._at[2], T, k, H, out.data_ptr(), _KINDS[dtype])
+              plan._at[3], T, k, H, out.data_ptr(), _KINDS[dtype])
     return out
 
 
@@ -258,7 +265,7 @@ def combine_backward(grad_out: torch.Tensor, y: torch.Tensor, plan: Plan, weight
     dw = (torch.empty if H else torch.zeros)((T, k), dtype=torch.float32, device=y.device)
     if dy.numel():
         _call("nvfp4_moe_combine_backward", y.device, grad_out.data_ptr(), _KINDS[grad_out.dtype], ldo, y.data_ptr(), _KINDS[y.dtype],
-              ld, weights.data_ptr(), plan._at[2], plan._at[0], T, plan.num_experts, k, H, dy.data_ptr(),
+              ld, weights.data_ptr(), plan._at[3], plan._at[0], T, plan.num_experts, k, H, dy.data_ptr(),
               dw.data_ptr())
     return dy, dw
 
@@ -275,7 +282,7 @@ def dispatch_nvfp4(x: torch.Tensor, plan: Plan):
     _same_device(x.device, plan)
     packed, scales = _new_operand(T * k, plan.most_tiles * 128, K, x.device)
     if T * k:
-        _call("nvfp4_moe_dispatch_nvfp4", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[2], plan._at[3],
+        _call("nvfp4_moe_dispatch_nvfp4", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[3], plan._at[4],
               plan._at[0], T, plan.num_experts, k, K, packed.data_ptr(), scales.data_ptr())
     return packed, scales
 
@@ -301,7 +308,7 @@ def _products(a, sfa, weights, plan: Plan, alpha):
             raise ValueError(f"alpha: expected a number or a contiguous float32 tensor of shape {(E,)}")
         _same_device(device, alpha)
         alphas, alpha = alpha.data_ptr(), 1.0
-    return ptrs + [plan._at[0], plan._at[1], alphas], float(alpha), R, E, N, K, device
+    return ptrs + [*plan._at[:3], alphas], float(alpha), R, E, N, K, device
 
 
 def expert_gemm(a, sfa, b, sfb, plan: Plan, alpha=1.0) -> torch.Tensor:

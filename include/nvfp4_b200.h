@@ -146,13 +146,14 @@ enum { NVFP4_F32 = 0, NVFP4_F16 = 1, NVFP4_BF16 = 2 };
 /* The plan of a batch, from the choices experts [T][k] (int32):
  *   offsets [E+1]  first row of each expert; offsets[E] rows are in use
  *   tiles   [E+1]  first 128-row tile of each expert (the sum of ceil(rows/128) of the experts before it)
+ *   wide_tiles [E+1]  the same for tiles of 256 rows
  *   rows    [T][k] row of a copy, -1: none
  *   slots   [T][k] 128 * tile + row in the tile: where the scales of the copy's row are, -1: none
  *   source  [T*k]  copy of a row, -1 behind the last one
  * all int32.  T, E, k > 0, k <= 32.  scratch: nvfp4_moe_plan_scratch(T, E, k) bytes (0 for up to 16384 copies: may be
  * NULL then), 4-byte aligned, not read after the call's kernels. */
-int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* rows, void* slots,
-                   void* source, void* scratch, void* stream);
+int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* wide_tiles, void* rows,
+                   void* slots, void* source, void* scratch, void* stream);
 long long nvfp4_moe_plan_scratch(int T, int E, int k);
 
 /* Router: weights [T][k] (fp32) and experts [T][k] (int32) of the k largest of each row of logits [T][E] (element type
@@ -161,8 +162,8 @@ long long nvfp4_moe_plan_scratch(int T, int E, int k);
  * whose byte in mask [T] (may be NULL) is 0 are never chosen and take no part in the sum; fewer than k candidates leave
  * experts -1 with weight 0.  k <= E. */
 int nvfp4_moe_route(const void* logits, int kind, long long ld, const void* mask, int T, int E, int k, int renormalize,
-                    void* weights, void* experts, void* offsets, void* tiles, void* rows, void* slots, void* source,
-                    void* scratch, void* stream);
+                    void* weights, void* experts, void* offsets, void* tiles, void* wide_tiles, void* rows, void* slots,
+                    void* source, void* scratch, void* stream);
 /* Its gradient: dlogits [T][E] (element type `kind`, contiguous) from dweights [T][k] (fp32), with the weights and
  * experts that the router returned; 0 for entries that took no part. */
 int nvfp4_moe_route_backward(const void* dweights, const void* logits, int kind, long long ld, const void* weights,
@@ -193,16 +194,17 @@ int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, const void* 
  * batched operand of nvfp4_gemm, alphas [E] fp32 or NULL, c [R][N]; rows behind the last copy become 0.
  * N % 128 == 0, K % 256 == 0; c 32-byte aligned, the operands 16-byte aligned. */
 int nvfp4_moe_gemm(const void* a, const void* sfa_sw, const void* b, const void* sfb_sw, const void* offsets,
-                   const void* tiles, const void* alphas, void* c, int R, int E, int N, int K, float alpha, void* stream);
+                   const void* tiles, const void* wide_tiles, const void* alphas, void* c, int R, int E, int N, int K,
+                   float alpha, void* stream);
 /* c[r] = fp16(silu(x) * y), x and y the products with b1[e] and b2[e], both times alpha * alphas[e]. */
 int nvfp4_moe_dual_gemm(const void* a, const void* sfa_sw, const void* b1, const void* sfb1_sw, const void* b2,
-                        const void* sfb2_sw, const void* offsets, const void* tiles, const void* alphas, void* c, int R,
-                        int E, int N, int K, float alpha, void* stream);
+                        const void* sfb2_sw, const void* offsets, const void* tiles, const void* wide_tiles,
+                        const void* alphas, void* c, int R, int E, int N, int K, float alpha, void* stream);
 /* The same with the result quantised, ready to be `a` of the next product of the same plan: c_packed [R][N/2], sfc_sw
  * [tiles][N/64][512]; bit for bit nvfp4_quantize_f16 of the fp16 rows. */
 int nvfp4_moe_dual_gemm_nvfp4(const void* a, const void* sfa_sw, const void* b1, const void* sfb1_sw, const void* b2,
-                              const void* sfb2_sw, const void* offsets, const void* tiles, const void* alphas,
-                              void* c_packed, void* sfc_sw, int R, int E, int N, int K, float alpha, void* stream);
+                              const void* sfb2_sw, const void* offsets, const void* tiles, const void* wide_tiles,
+                              const void* alphas, void* c_packed, void* sfc_sw, int R, int E, int N, int K, float alpha, void* stream);
 
 /* Last device-side status code of device `dev` (0 = none); clear != 0 resets it.
  * Call after synchronising the stream.  No counterpart in the reference, whose kernels spin

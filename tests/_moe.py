@@ -11,10 +11,10 @@ TINY = {torch.float32: 2.0 ** -150, torch.float16: 2.0 ** -25, torch.bfloat16: 2
 
 
 def plan_ref(experts: torch.Tensor, E: int):
-    """offsets, tiles, rows, slots, source of int choices [T, k], by counting (CPU, int64)."""
+    """offsets, tiles, wide_tiles, rows, slots, source of int choices [T, k], by counting (CPU, int64)."""
     ids = experts.cpu().reshape(-1).tolist()
     by = [[i for i, e in enumerate(ids) if e == x] for x in range(E)]
-    offsets, tiles = [0], [0]
+    offsets, tiles, wide = [0], [0], [0]
     rows, slots, source = [-1] * len(ids), [-1] * len(ids), []
     for copies in by:
         for n, i in enumerate(copies):
@@ -22,14 +22,15 @@ def plan_ref(experts: torch.Tensor, E: int):
         source += copies
         offsets.append(offsets[-1] + len(copies))
         tiles.append(tiles[-1] + (len(copies) + 127) // 128)
+        wide.append(wide[-1] + (len(copies) + 255) // 256)
     source += [-1] * (len(ids) - len(source))
     t = lambda v: torch.tensor(v, dtype=torch.int64)  # noqa: E731
-    return t(offsets), t(tiles), t(rows).view(experts.shape), t(slots).view(experts.shape), t(source)
+    return t(offsets), t(tiles), t(wide), t(rows).view(experts.shape), t(slots).view(experts.shape), t(source)
 
 
 def check_plan(plan, experts, E):
     assert (plan.num_tokens, plan.top_k, plan.num_experts) == (*experts.shape, E)
-    for name, want in zip(("offsets", "tiles", "rows", "slots", "source"), plan_ref(experts, E)):
+    for name, want in zip(("offsets", "tiles", "wide_tiles", "rows", "slots", "source"), plan_ref(experts, E)):
         got = getattr(plan, name)
         assert got.dtype == torch.int32 and torch.equal(got.cpu().long(), want), name
 

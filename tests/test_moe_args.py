@@ -5,7 +5,7 @@ import torch
 
 def test_c_entries_reject_bad_arguments(lib):
     P = 32                                                # stands for an aligned pointer; nothing is read
-    plan = (P,) * 6                                       # five tables and the scratch
+    plan = (P,) * 7                                       # six tables and the scratch
     assert lib.nvfp4_moe_plan(None, 4, 4, 2, *plan, None) == -1
     assert lib.nvfp4_moe_plan(P, 0, 4, 2, *plan, None) == -2
     assert lib.nvfp4_moe_plan(P, 4, 0, 2, *plan, None) == -2
@@ -13,7 +13,7 @@ def test_c_entries_reject_bad_arguments(lib):
     assert lib.nvfp4_moe_plan(P, 4, 64, 33, *plan, None) == -6
     assert lib.nvfp4_moe_plan(P, 1 << 30, 4, 2, *plan, None) == -6       # copies are counted in 32 bits
     assert lib.nvfp4_moe_plan_scratch(2048, 64, 8) == 0 and lib.nvfp4_moe_plan_scratch(2049, 64, 8) > 0
-    assert lib.nvfp4_moe_plan(P, 2049, 64, 8, *plan[:5], None, None) == -1
+    assert lib.nvfp4_moe_plan(P, 2049, 64, 8, *plan[:6], None, None) == -1
     route = lambda kind=0, ld=8, T=4, E=8, k=2, logits=P: lib.nvfp4_moe_route(  # noqa: E731
         logits, kind, ld, None, T, E, k, 1, P, P, *plan, None)
     assert route(logits=None) == -1
@@ -32,13 +32,13 @@ def test_c_entries_reject_bad_arguments(lib):
         x, kind, ld, P, P, P, 4, 8, 2, K, codes, P, None)
     assert dq(x=None) == -1 and dq(K=96, ld=96) == -3 and dq(x=8) == -5 and dq(ld=65) == -5 and dq(codes=4) == -5
     assert dq(kind=3) == -6
-    gemm = lambda a=P, N=128, K=256, R=8, E=4, c=P, off=P, al=None: lib.nvfp4_moe_gemm(  # noqa: E731
-        a, P, P, P, off, P, al, c, R, E, N, K, 1.0, None)
-    assert gemm(a=None) == -1 and gemm(off=None) == -1
+    gemm = lambda a=P, N=128, K=256, R=8, E=4, c=P, off=P, al=None, wide=P: lib.nvfp4_moe_gemm(  # noqa: E731
+        a, P, P, P, off, P, wide, al, c, R, E, N, K, 1.0, None)
+    assert gemm(a=None) == -1 and gemm(off=None) == -1 and gemm(wide=None) == -1
     assert gemm(N=64) == -4 and gemm(K=128) == -3 and gemm(R=0) == -2 and gemm(E=0) == -2
     assert gemm(a=8) == -5 and gemm(c=16) == -5 and gemm(al=2) == -5
-    assert lib.nvfp4_moe_dual_gemm(P, P, P, P, None, P, P, P, None, P, 8, 4, 128, 256, 1.0, None) == -1
-    assert lib.nvfp4_moe_dual_gemm_nvfp4(P, P, P, P, P, P, P, P, None, P, None, 8, 4, 128, 256, 1.0, None) == -1
+    assert lib.nvfp4_moe_dual_gemm(P, P, P, P, None, P, P, P, P, None, P, 8, 4, 128, 256, 1.0, None) == -1
+    assert lib.nvfp4_moe_dual_gemm_nvfp4(P, P, P, P, P, P, P, P, P, None, P, None, 8, 4, 128, 256, 1.0, None) == -1
 
 
 def test_python_entries_take_cuda_tensors_of_the_documented_types():
