@@ -86,7 +86,9 @@ def load() -> ctypes.CDLL:
     lib.nvfp4_moe_dispatch.argtypes = [vp, i, ll, vp, vp, i, i, i, i, vp, vp]
     lib.nvfp4_moe_combine.argtypes = [vp, i, ll, vp, vp, i, i, i, vp, i, vp]
     lib.nvfp4_moe_combine_backward.argtypes = [vp, i, ll, vp, i, ll, vp, vp, vp, i, i, i, i, vp, vp, vp]
-    lib.nvfp4_moe_dispatch_nvfp4.argtypes = [vp, i, ll, vp, vp, vp, i, i, i, i, vp, vp, vp]
+    lib.nvfp4_moe_dispatch_nvfp4.argtypes = [vp, i, ll, vp, vp, vp, vp, vp, i, i, i, i, vp, vp, vp, vp]
+    lib.nvfp4_moe_dispatch_scratch.argtypes = [i, i, i]
+    lib.nvfp4_moe_dispatch_scratch.restype = ll
     lib.nvfp4_moe_gemm.argtypes = [vp] * 9 + [i, i, i, i, f, vp]
     lib.nvfp4_moe_dual_gemm.argtypes = [vp] * 11 + [i, i, i, i, f, vp]
     lib.nvfp4_moe_dual_gemm_nvfp4.argtypes = [vp] * 12 + [i, i, i, i, f, vp]

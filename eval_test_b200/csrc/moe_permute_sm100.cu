@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* __restrict
 
 // KU rows' loads of U vectors each are in flight at a time.  `pitch`: bytes between rows of y.
 template <typename TI, typename TO, int VN, int KU, int U, bool WEIGHTED>
-__global__ void __launch_bounds__(256, U == 2 ? 3 : 4) combine_kernel(const TI* __restrict__ y, unsigned pitch, const float* __restrict__ weights,
+__global__ void __launch_bounds__(256, U >= 2 ? 3 : 4) combine_kernel(const TI* __restrict__ y, unsigned pitch, const float* __restrict__ weights,
                                                          TO* __restrict__ out, int row_vecs, const PermuteArgs p) {
     pdl_wait();
     pdl_launch();
@@ -231,12 +231,15 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* __re
     zero_tail(reinterpret_cast<typename Bits<VN * sizeof(TI)>::type*>(dy), row_vecs, p);
 }
 
-// One thread per 32 elements of a token: quantised once, their codes (16 bytes) and scale bytes stored for each of the
-// token's rows.  Two neighbouring lanes hold the four k-blocks of one 4-byte group of a scale atom (K % 64 == 0).  The
-// scale atoms follow the experts' 128-row tiles: slots[t][j] is the row with every expert padded to whole tiles.
-template <int KIND>
+// One thread per 32 elements of a token: quantised once, their codes (16 bytes) stored for each of the token's rows.
+// The scale atoms follow the experts' 128-row tiles: slots[t][j] is the row with every expert padded to whole tiles.
+// TABLE = false: the scale bytes are stored for each row, too; two neighbouring lanes hold the four k-blocks of one
+// 4-byte group of an atom (K % 64 == 0).  TABLE = true: they go to a row of `table` per token, from where
+// gather_scales_kernel makes whole atoms: 4-byte stores 512 bytes apart took as long as everything else together
+// (16384 tokens x 8 x 4096: 130 us, 90 us with the table).
+template <int KIND, bool TABLE>
 __global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* __restrict__ x, long long ld, const int* __restrict__ slots,
-                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ sf_sw,
+                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                              const PermuteArgs p) {
     using T = typename ElemOf<KIND>::type;
     pdl_wait();
@@ -261,8 +264,11 @@ __global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* __restr
         uint4 w;
         uint32_t s = quantize_block16(xs, w.x, w.y);
         s |= quantize_block16(xs + 16, w.z, w.w) << 8;
-        // (n is even, so the two lanes of a group are in range together)
-        s |= __shfl_down_sync(0xffffffffu, s, 1) << 16;
+        if (TABLE) {
+            if (in) reinterpret_cast<uint16_t*>(scales)[i] = (uint16_t)s;
+        } else {
+            s |= __shfl_down_sync(0xffffffffu, s, 1) << 16;   // (n is even: the two lanes of a group are in range together)
+        }
         if (!in) continue;
         const int* rows = p.rows + t * p.k;
         uint8_t* dst = codes + (long long)c * 16;
@@ -270,14 +276,49 @@ __global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* __restr
             const int row = __ldg(rows + j);
             if (row < 0) continue;
             *reinterpret_cast<uint4*>(dst + (long long)row * units * 16) = w;
-            if ((lane & 1) == 0) {
+            if (!TABLE && (lane & 1) == 0) {
                 const int slot = __ldg(slots + t * p.k + j);
                 const long long atom = (long long)(slot >> 7) * (units / 2) + c / 2;
-                *reinterpret_cast<uint32_t*>(sf_sw + atom * 512 + (slot & 31) * 16 + ((slot & 127) >> 5) * 4) = s;
+                *reinterpret_cast<uint32_t*>(scales + atom * 512 + (slot & 31) * 16 + ((slot & 127) >> 5) * 4) = s;
             }
         }
     }
     zero_tail(reinterpret_cast<uint4*>(codes), units, p);
+}
+
+// The scale atoms of one 128-row tile from the tokens' scale rows: a warp makes four atoms (256 elements of K) at a time,
+// lane i the 16 bytes of the rows i, i + 32, i + 64, i + 96 in each.  Rows that do not exist get zeros.
+__global__ void __launch_bounds__(256) gather_scales_kernel(const uint8_t* __restrict__ table, const int* __restrict__ source,
+                                                            const int* __restrict__ offsets, const int* __restrict__ tiles,
+                                                            uint8_t* __restrict__ sf_sw, int E, int k, int K) {
+    __shared__ int expert;
+    pdl_wait();
+    pdl_launch();
+    const int tile = blockIdx.x;
+    if (tile >= __ldg(tiles + E)) return;
+    for (int e = threadIdx.x; e < E; e += blockDim.x)
+        if (__ldg(tiles + e) <= tile && tile < __ldg(tiles + e + 1)) expert = e;
+    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int row0 = __ldg(offsets + expert) + (tile - __ldg(tiles + expert)) * 128, end = __ldg(offsets + expert + 1);
+    long long token[4];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const int row = row0 + q * 32 + lane;
+        token[q] = row < end ? __ldg(source + row) / k : -1;
+    }
+    const int chunks = K / 256;
+    for (int c = blockIdx.y * 8 + warp; c < chunks; c += gridDim.y * 8) {
+        uint4 w[4];
+#pragma unroll
+        for (int q = 0; q < 4; q++)
+            w[q] = token[q] >= 0 ? __ldg(reinterpret_cast<const uint4*>(table + token[q] * (K / 16)) + c) : make_uint4(0u, 0u, 0u, 0u);
+        uint4* dst = reinterpret_cast<uint4*>(sf_sw + ((long long)tile * (K / 64) + c * 4) * 512) + lane;
+        dst[0] = make_uint4(w[0].x, w[1].x, w[2].x, w[3].x);
+        dst[32] = make_uint4(w[0].y, w[1].y, w[2].y, w[3].y);
+        dst[64] = make_uint4(w[0].z, w[1].z, w[2].z, w[3].z);
+        dst[96] = make_uint4(w[0].w, w[1].w, w[2].w, w[3].w);
+    }
 }
 
 // Vectors per lane: one as long as that gives every SM a few warps, else U.
@@ -387,7 +428,8 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
             using std::integral_constant;
             auto go_width = [&](auto vn) {
                 if (spread(T, row_vecs, dev)) return go(vn, integral_constant<int, 8>(), integral_constant<int, 1>());
-                if (k <= 2) return go(vn, integral_constant<int, 2>(), integral_constant<int, 2>());
+                // (of two rows, as many vectors as eight rows have: 4096 x 2 x 2048 fp32 17.3 us with four against 19.0 with two)
+                if (k <= 2) return go(vn, integral_constant<int, 2>(), integral_constant<int, VN == 4 ? 4 : 2>());
                 if (k <= 4) return go(vn, integral_constant<int, 4>(), integral_constant<int, 2>());
                 return go(vn, integral_constant<int, 8>(), integral_constant<int, 1>());
             };
@@ -421,8 +463,10 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
             const bool wide = H % VN == 0 && ld % VN == 0 && ldo % VN == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)dy % 16 == 0 &&
                               (uintptr_t)dout % O == 0;
             const int row_vecs = wide ? H / VN : H;
-            // a warp per token where its lanes take at most four vectors each
-            const bool warp = row_vecs <= 128;
+            // a warp per token where its lanes take at most four vectors each, and for few choices where there are tokens
+            // enough for that (bf16, 4096 wide, a warp against a block: 16384 x 1 65 against 86 us, 8192 x 4 98 / 105; with
+            // eight rows in registers a warp's loads no longer cover its stores: 16384 x 8 372 / 351)
+            const bool warp = row_vecs <= 128 || (k <= 4 && T >= 16 * sm_count(dev));
             const int grid = grid_for((long long)T * (warp ? 32 : 256), dev);
             auto go = [&](auto vn, auto group, auto ku, auto u) {
                 return launch_dependent(
@@ -444,22 +488,43 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
     });
 }
 
-extern "C" int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, const void* rows, const void* slots,
-                                        const void* offsets, int T, int E, int k, int K, void* packed, void* sf_sw, void* stream) {
-    if (!x || !rows || !slots || !offsets || !packed || !sf_sw) return NVFP4_ERR_NULL;
+extern "C" long long nvfp4_moe_dispatch_scratch(int T, int k, int K) {
+    // a second launch pays for many elements (bf16, without and with: 8192 x 2 x 4096 22 against 24.5 us, 8192 x 4 x 4096
+    // 32 / 31, 4096 x 6 x 7168 38 / 36, 16384 x 8 x 4096 130 / 90)
+    return T > 0 && k > 0 && K > 0 && K % 256 == 0 && (long long)T * k * K >= (160ll << 20) ? (long long)T * (K / 16) : 0;
+}
+
+extern "C" int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, const void* offsets, const void* tiles,
+                                        const void* rows, const void* slots, const void* source, int T, int E, int k, int K,
+                                        void* packed, void* sf_sw, void* scratch, void* stream) {
+    if (!x || !offsets || !tiles || !rows || !slots || !source || !packed || !sf_sw) return NVFP4_ERR_NULL;
     if (!kind_ok(kind)) return NVFP4_ERR_UNSUPPORTED;
     int rc = check_sizes(T, k, K, ld);
     if (rc) return rc;
     if (E <= 0) return NVFP4_ERR_SHAPE;
     if (K % 64 != 0) return NVFP4_ERR_K_MULTIPLE;
-    if (((uintptr_t)x & 15) || ld * elem_bytes(kind) % 16 || ((uintptr_t)packed & 15) || ((uintptr_t)sf_sw & 3)) return NVFP4_ERR_ALIGN;
+    const bool table = nvfp4_moe_dispatch_scratch(T, k, K) > 0;
+    if (table && !scratch) return NVFP4_ERR_NULL;
+    if (((uintptr_t)x & 15) || ld * elem_bytes(kind) % 16 || ((uintptr_t)packed & 15) || ((uintptr_t)sf_sw & 15) ||
+        (table && ((uintptr_t)scratch & 15)))
+        return NVFP4_ERR_ALIGN;
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;
     const PermuteArgs p{(const int*)rows, (const int*)offsets + E, T, k, K};
     const int grid = grid_for((long long)T * (K / 32), dev);
     cudaStream_t st = (cudaStream_t)stream;
-    auto kernel = kind == NVFP4_F32   ? dispatch_quant_kernel<NVFP4_F32>
-                  : kind == NVFP4_F16 ? dispatch_quant_kernel<NVFP4_F16>
-                                      : dispatch_quant_kernel<NVFP4_BF16>;
-    return launch_dependent(kernel, grid, 256, 0, 0, st, x, ld, (const int*)slots, (uint8_t*)packed, (uint8_t*)sf_sw, p);
+    auto go = [&](auto with_table) {
+        constexpr bool TB = decltype(with_table)::value;
+        auto kernel = kind == NVFP4_F32   ? dispatch_quant_kernel<NVFP4_F32, TB>
+                      : kind == NVFP4_F16 ? dispatch_quant_kernel<NVFP4_F16, TB>
+                                          : dispatch_quant_kernel<NVFP4_BF16, TB>;
+        return launch_dependent(kernel, grid, 256, 0, 0, st, x, ld, (const int*)slots, (uint8_t*)packed, (uint8_t*)(TB ? scratch : sf_sw), p);
+    };
+    if (!table) return go(std::false_type());
+    if ((rc = go(std::true_type()))) return rc;
+    // blocks for the most tiles that the copies can fill; those without a tile end at once
+    const long long copies = (long long)T * k, active = copies < E ? copies : E;
+    const dim3 tiles_grid((unsigned)(active + (copies - active) / 128), (K / 256 + 7) / 8 < 4 ? (K / 256 + 7) / 8 : 4);
+    return launch_dependent(gather_scales_kernel, tiles_grid, 256, 0, 0, st, (const uint8_t*)scratch, (const int*)source, (const int*)offsets,
+                            (const int*)tiles, (uint8_t*)sf_sw, E, k, K);
 }

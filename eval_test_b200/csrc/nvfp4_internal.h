@@ -19,9 +19,9 @@ unsigned long long wait_budget_ns();
 // Launches with programmatic dependent launch (and in clusters of `cluster` CTAs where that is not 0): the kernels of a
 // layer are short, and the start of each then hides behind the end of the one before it.
 template <typename... P, typename... A>
-int launch_dependent(void (*kernel)(P...), int grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
+int launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t st, const A&... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;

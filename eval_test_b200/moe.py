@@ -33,34 +33,23 @@ _KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 class Plan:
     """How the copies of a batch are sorted (``nvfp4_moe_plan``).  One int32 buffer on the batch's device holds its six
     tables; the views are made when they are asked for (a call of the layer needs only their addresses)."""
-    __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "_at")
+    __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "num_copies", "most_tiles", "device", "_at")
 
-    def __init__(self, num_tokens: int, top_k: int, num_experts: int, device: torch.device):
+    def __init__(self, num_tokens: int, top_k: int, num_experts: int, device: torch.device, more: int = 0):
         n, e = num_tokens * top_k, num_experts + 1
-        # behind the tables: the copies per expert of each block of a large sort
-        size = 3 * e + 3 * n + (_lib.load().nvfp4_moe_plan_scratch(num_tokens, num_experts, top_k) // 4 if n > 4096 else 0)
+        # behind the tables: the copies per expert of each block of a large sort, then `more` words for the caller
+        scratch = _lib.load().nvfp4_moe_plan_scratch(num_tokens, num_experts, top_k) // 4 if n > 4096 else 0
+        size = 3 * e + 3 * n + scratch + more
         # (no copies: nothing is launched, and every expert starts at row 0)
         self.buffer = torch.empty(size, dtype=torch.int32, device=device) if n else torch.zeros(size, dtype=torch.int32, device=device)
-        self.num_tokens, self.top_k, self.num_experts = num_tokens, top_k, num_experts
+        self.num_tokens, self.top_k, self.num_experts, self.num_copies, self.device = num_tokens, top_k, num_experts, n, device
+        # 128-row tiles that this many copies can fill at most, whatever their experts
+        active = n if n < num_experts else num_experts
+        self.most_tiles = active + (n - active) // 128
         base = self.buffer.data_ptr()
         rows = base + 12 * e
-        n *= 4
-        self._at = (base, base + 4 * e, base + 8 * e, rows, rows + n, rows + 2 * n, rows + 3 * n)
-
-    @property
-    def device(self) -> torch.device:
-        return self.buffer.device
-
-    @property
-    def num_copies(self) -> int:
-        return self.num_tokens * self.top_k
-
-    @property
-    def most_tiles(self) -> int:
-        """128-row tiles that this many copies can fill at most, whatever their experts."""
-        copies = self.num_tokens * self.top_k
-        active = min(copies, self.num_experts)
-        return active + (copies - active) // 128
+        # addresses: offsets, tiles, wide_tiles, rows, slots, source, scratch
+        self._at = (base, base + 4 * e, base + 8 * e, rows, rows + 4 * n, rows + 8 * n, rows + 12 * n)
 
     def _per_expert(self, i: int) -> torch.Tensor:
         e = self.num_experts + 1
@@ -144,12 +133,28 @@ def _call(entry: str, device: torch.device, *args) -> None:
         _lib.check(code, entry)
 
 
-def _new_operand(rows: int, tile_rows: int, K: int, device):
+def _operand(t: torch.Tensor, rows: int, k2: int, L: int, name: str) -> int:
+    if t.shape == (rows, k2, L) and t.element_size() == 1 and t.is_cuda:
+        a, b, c = t.stride()
+        if a == k2 and b == 1 and (L == 1 or c == rows * k2):
+            return t.data_ptr()
+    return _args.operand_ptr(t, rows, k2, L, name)       # (strides of dimensions of size 1 may be others; else it raises)
+
+
+def _scales(t: torch.Tensor, rows: int, K: int, L: int, name: str) -> int:
+    R, Kb = rows // 128, K // 64
+    if t.shape == (32, 4, R, 4, Kb, L) and t.element_size() == 1 and t.is_cuda:
+        *inner, outer = t.stride()
+        if inner == [16, 4, Kb * 512, 1, 512] and (L == 1 or outer == R * Kb * 512):
+            return t.data_ptr()
+    return _args.scales_ptr(t, rows, K, L, name)
+
+
+def _new_operand(like: torch.Tensor, rows: int, tile_rows: int, K: int):
     """An operand ``[rows, K/2, 1]`` and the 6-D swizzled view of the scales of ``tile_rows`` rows, not initialised."""
-    packed = torch.empty((rows, K // 2, 1), dtype=torch.float4_e2m1fn_x2, device=device)
-    scales = torch.empty_strided((32, 4, tile_rows // 128, 4, K // 64, 1), F.permuted_strides(tile_rows, K),
-                                 dtype=torch.float8_e4m3fn, device=device)
-    return packed, scales
+    R, Kb = tile_rows // 128, K // 64
+    return (like.new_empty((rows, K // 2, 1), dtype=torch.float4_e2m1fn_x2),
+            like.new_empty_strided((32, 4, R, 4, Kb, 1), (16, 4, Kb * 512, 1, 512, R * Kb * 512), dtype=torch.float8_e4m3fn))
 
 
 def plan(experts: torch.Tensor, num_experts: int) -> Plan:
@@ -185,12 +190,16 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torc
         if mask.dtype != torch.bool or mask.shape != (T,) or not mask.is_contiguous():
             raise ValueError(f"mask: expected a contiguous bool tensor of shape {(T,)}")
         _same_device(device, mask)
-    weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
-    experts = torch.empty((T, top_k), dtype=torch.int32, device=device)
-    p = Plan(T, top_k, E, device)
+    # the weights and the choices lie behind the plan's tables (one allocation: each costs as much as a launch)
+    n = T * top_k
+    p = Plan(T, top_k, E, device, 2 * n)
+    at = p.buffer.shape[0] - 2 * n
+    weights = p.buffer.view(torch.float32).as_strided((T, top_k), (top_k, 1), at)
+    experts = p.buffer.as_strided((T, top_k), (top_k, 1), at + n)
     if T:
+        address = p._at[0] + 4 * at
         _call("nvfp4_moe_route", device, logits.data_ptr(), _KINDS[logits.dtype], ld, None if mask is None else mask.data_ptr(),
-              T, E, top_k, int(renormalize), weights.data_ptr(), experts.data_ptr(), *p._at)
+              T, E, top_k, int(renormalize), address, address + 4 * n, *p._at)
     return Routing(weights, experts, p)
 
 
@@ -208,7 +217,7 @@ def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, weights: to
     _choices(weights, "weights", torch.float32, (T, k))
     _choices(grad_weights, "grad_weights", torch.float32, (T, k))
     _same_device(logits.device, weights, experts, grad_weights)
-    out = torch.empty((T, E), dtype=logits.dtype, device=logits.device)
+    out = logits.new_empty((T, E))
     if T:
         _call("nvfp4_moe_route_backward", logits.device, grad_weights.data_ptr(), logits.data_ptr(), _KINDS[logits.dtype], ld,
               weights.data_ptr(), experts.data_ptr(), T, E, k, int(renormalize), out.data_ptr())
@@ -221,7 +230,7 @@ def dispatch(x: torch.Tensor, plan: Plan) -> torch.Tensor:
     ld = _matrix(x, "x", T)
     H = x.shape[1]
     _same_device(x.device, plan)
-    out = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
+    out = x.new_empty((T * k, H))
     if out.numel():
         _call("nvfp4_moe_dispatch", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[3], plan._at[0], T,
               plan.num_experts, k, H, out.data_ptr())
@@ -245,8 +254,7 @@ def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dt
     if weights is not None:
         _choices(weights, "weights", torch.float32, (T, k))
     _same_device(y.device, plan, weights)
-    make = torch.empty if k else torch.zeros
-    out = make((T, H), dtype=dtype, device=y.device)
+    out = y.new_empty((T, H), dtype=dtype) if k else y.new_zeros((T, H), dtype=dtype)
     if out.numel() and k:
         _call("nvfp4_moe_combine", y.device, y.data_ptr(), _KINDS[y.dtype], ld, None if weights is None else weights.data_ptr(),
               plan._at[3], T, k, H, out.data_ptr(), _KINDS[dtype])
@@ -261,8 +269,8 @@ def combine_backward(grad_out: torch.Tensor, y: torch.Tensor, plan: Plan, weight
     H = y.shape[1]
     _choices(weights, "weights", torch.float32, (T, k))
     _same_device(y.device, grad_out, plan, weights)
-    dy = torch.empty((T * k, H), dtype=y.dtype, device=y.device)
-    dw = (torch.empty if H else torch.zeros)((T, k), dtype=torch.float32, device=y.device)
+    dy = y.new_empty((T * k, H))
+    dw = torch.empty_like(weights) if H else torch.zeros_like(weights)
     if dy.numel():
         _call("nvfp4_moe_combine_backward", y.device, grad_out.data_ptr(), _KINDS[grad_out.dtype], ldo, y.data_ptr(), _KINDS[y.dtype],
               ld, weights.data_ptr(), plan._at[3], plan._at[0], T, plan.num_experts, k, H, dy.data_ptr(),
@@ -273,17 +281,20 @@ def combine_backward(grad_out: torch.Tensor, y: torch.Tensor, plan: Plan, weight
 def dispatch_nvfp4(x: torch.Tensor, plan: Plan):
     """``dispatch`` with the rows quantised as ``quantize.quantize_operand`` does: ``x`` [T, K] -> (operand
     ``[T * k, K/2, 1]`` float4_e2m1fn_x2, 6-D swizzled scales of the experts' 128-row tiles, ``plan.most_tiles`` of them).
-    Scale bytes of rows that do not exist are not written.  K is a multiple of 64."""
+    Scale bytes of rows that do not exist have no meaning.  K is a multiple of 64."""
     T, k = plan.num_tokens, plan.top_k
     ld = _matrix(x, "x", T)
     K = x.shape[1]
     if K % 64 or not K:
         raise ValueError(f"x: the width has to be a multiple of 64, got {K}")
     _same_device(x.device, plan)
-    packed, scales = _new_operand(T * k, plan.most_tiles * 128, K, x.device)
+    packed, scales = _new_operand(x, T * k, plan.most_tiles * 128, K)
     if T * k:
-        _call("nvfp4_moe_dispatch_nvfp4", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[3], plan._at[4],
-              plan._at[0], T, plan.num_experts, k, K, packed.data_ptr(), scales.data_ptr())
+        scratch = _lib.load().nvfp4_moe_dispatch_scratch(T, k, K) if T * k > 1024 else 0
+        table = x.new_empty(scratch, dtype=torch.uint8) if scratch else None
+        offsets, tiles, _, rows, slots, source, _ = plan._at
+        _call("nvfp4_moe_dispatch_nvfp4", x.device, x.data_ptr(), _KINDS[x.dtype], ld, offsets, tiles, rows, slots, source, T,
+              plan.num_experts, k, K, packed.data_ptr(), scales.data_ptr(), table.data_ptr() if scratch else None)
     return packed, scales
 
 
@@ -298,9 +309,9 @@ def _products(a, sfa, weights, plan: Plan, alpha):
         raise ValueError(f"a: K has to be a multiple of 256, got {K}")
     if N % 128 or not N:
         raise ValueError(f"b: N has to be a multiple of 128, got {N}")
-    ptrs = [_args.operand_ptr(a, R, K // 2, 1, "a"), _args.scales_ptr(sfa, plan.most_tiles * 128, K, 1, "sfa")]
+    ptrs = [_operand(a, R, K // 2, 1, "a"), _scales(sfa, plan.most_tiles * 128, K, 1, "sfa")]
     for i in range(0, len(weights), 2):
-        ptrs += [_args.operand_ptr(weights[i], N, K // 2, E, "b"), _args.scales_ptr(weights[i + 1], N, K, E, "sfb")]
+        ptrs += [_operand(weights[i], N, K // 2, E, "b"), _scales(weights[i + 1], N, K, E, "sfb")]
     _same_device(device, sfa, *weights, plan)
     alphas = None
     if isinstance(alpha, torch.Tensor):
@@ -316,7 +327,7 @@ def expert_gemm(a, sfa, b, sfb, plan: Plan, alpha=1.0) -> torch.Tensor:
     ``dispatch_nvfp4`` or ``expert_dual_gemm_nvfp4`` returns them, ``b`` [N, K/2, E] with its 6-D scales; ``alpha`` a number
     or a float32 tensor [E], the experts' global scales.  N is a multiple of 128, K of 256."""
     ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b, sfb), plan, alpha)
-    c = torch.empty((R, N), dtype=torch.float16, device=device)
+    c = a.new_empty((R, N), dtype=torch.float16)
     if R:
         _call("nvfp4_moe_gemm", device, *ptrs, c.data_ptr(), R, E, N, K, alpha)
     return c
@@ -326,7 +337,7 @@ def expert_dual_gemm(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0) -> torch
     """``fp16(silu(alpha_e * a[r] @ b1_e^T) * (alpha_e * a[r] @ b2_e^T))`` -> fp16 [T * k, N]; arguments as for
     ``expert_gemm``."""
     ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
-    c = torch.empty((R, N), dtype=torch.float16, device=device)
+    c = a.new_empty((R, N), dtype=torch.float16)
     if R:
         _call("nvfp4_moe_dual_gemm", device, *ptrs, c.data_ptr(), R, E, N, K, alpha)
     return c
@@ -336,7 +347,7 @@ def expert_dual_gemm_nvfp4(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0):
     """``expert_dual_gemm`` with its rows quantised to NVFP4, bit for bit what quantising the fp16 rows gives -> (operand
     ``[T * k, N/2, 1]``, 6-D scales): ``a`` and ``sfa`` of the next product of the same plan."""
     ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
-    packed, scales = _new_operand(R, plan.most_tiles * 128, N, device)
+    packed, scales = _new_operand(a, R, plan.most_tiles * 128, N)
     if R:
         _call("nvfp4_moe_dual_gemm_nvfp4", device, *ptrs, packed.data_ptr(), scales.data_ptr(), R, E, N, K, alpha)
     return packed, scales

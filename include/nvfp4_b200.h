@@ -183,11 +183,14 @@ int nvfp4_moe_combine_backward(const void* dout, int out_kind, long long ldo, co
                                void* dy, void* dweights, void* stream);
 
 /* nvfp4_moe_dispatch with the rows quantised as nvfp4_quantize_* does: packed [T*k][K/2] (rows behind the last copy
- * become 0) and sf_sw, the scale atoms [tiles][K/64][512] of every expert's own 128-row tiles (bytes of rows that do
- * not exist are left as they are).  At most min(T*k, E) + (T*k - min(T*k, E)) / 128 tiles.  K % 64 == 0; x and its pitch
- * 16-byte aligned. */
-int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, const void* rows, const void* slots, const void* offsets,
-                             int T, int E, int k, int K, void* packed, void* sf_sw, void* stream);
+ * become 0) and sf_sw, the scale atoms [tiles][K/64][512] of every expert's own 128-row tiles (the bytes of rows that do
+ * not exist have no meaning).  At most min(T*k, E) + (T*k - min(T*k, E)) / 128 tiles.  K % 64 == 0; x, its pitch, packed
+ * and sf_sw 16-byte aligned.  scratch: nvfp4_moe_dispatch_scratch(T, k, K) bytes, 16-byte aligned, not read after the
+ * call's kernels (NULL where that is 0). */
+int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, const void* offsets, const void* tiles,
+                             const void* rows, const void* slots, const void* source, int T, int E, int k, int K,
+                             void* packed, void* sf_sw, void* scratch, void* stream);
+long long nvfp4_moe_dispatch_scratch(int T, int k, int K);
 
 /* The experts' products: c[r] = fp16(alpha * alphas[e] * (a*sfa)[r] @ (b*sfb)[e]^T) for every row r of expert e;
  * a [R][K/2] and sfa_sw as nvfp4_moe_dispatch_nvfp4 leaves them (R = T*k), b [E][N][K/2] with swizzled scales as one

@@ -28,10 +28,13 @@ def test_c_entries_reject_bad_arguments(lib):
     assert comb(y=None) == -1 and comb(kind=5) == -6 and comb(ok=5) == -6 and comb(k=0) == -2
     cb = lambda d=P, kind=0, w=P: lib.nvfp4_moe_combine_backward(d, 0, 8, P, kind, 8, w, P, P, 4, 8, 2, 8, P, P, None)  # noqa: E731
     assert cb(d=None) == -1 and cb(w=None) == -1 and cb(kind=7) == -6
-    dq = lambda x=P, K=64, ld=64, kind=2, codes=P: lib.nvfp4_moe_dispatch_nvfp4(  # noqa: E731
-        x, kind, ld, P, P, P, 4, 8, 2, K, codes, P, None)
-    assert dq(x=None) == -1 and dq(K=96, ld=96) == -3 and dq(x=8) == -5 and dq(ld=65) == -5 and dq(codes=4) == -5
+    dq = lambda x=P, K=64, ld=64, kind=2, codes=P, T=4, scratch=None: lib.nvfp4_moe_dispatch_nvfp4(  # noqa: E731
+        x, kind, ld, P, P, P, P, P, T, 8, 2, K, codes, P, scratch, None)
+    assert dq(x=None) == -1 and dq(K=96, ld=96) == -3 and dq(x=8) == -5 and dq(ld=65) == -5 and dq(codes=8) == -5
     assert dq(kind=3) == -6
+    assert lib.nvfp4_moe_dispatch_scratch(1 << 18, 2, 256) == 0 and lib.nvfp4_moe_dispatch_scratch(1 << 20, 2, 256) == 1 << 24
+    assert lib.nvfp4_moe_dispatch_scratch(1 << 20, 2, 320) == 0
+    assert dq(T=1 << 20, K=256, ld=256) == -1 and dq(T=1 << 20, K=256, ld=256, scratch=8) == -5
     gemm = lambda a=P, N=128, K=256, R=8, E=4, c=P, off=P, al=None, wide=P: lib.nvfp4_moe_gemm(  # noqa: E731
         a, P, P, P, off, P, wide, al, c, R, E, N, K, 1.0, None)
     assert gemm(a=None) == -1 and gemm(off=None) == -1 and gemm(wide=None) == -1

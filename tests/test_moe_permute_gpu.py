@@ -8,8 +8,9 @@ from _moe import EPS32, STEP, TINY, choices
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+# T, E, k, H; the last two: a warp per token, and four vectors of two rows at a time
 SIZES = [(1, 1, 1, 8), (1, 64, 8, 4096), (5, 3, 2, 1), (40, 7, 3, 100), (33, 16, 4, 1001), (300, 8, 2, 64), (129, 40, 10, 1032),
-         (2, 5, 5, 8200)]
+         (2, 5, 5, 8200), (2500, 3, 2, 1304), (2400, 9, 3, 1040)]
 
 
 def _normal(shape, dtype, seed):
@@ -132,7 +133,8 @@ def test_of_no_tokens_and_no_columns():
     assert dy.shape == (8, 0) and not dw.any()
 
 
-@pytest.mark.parametrize("T,E,k,K", [(1, 1, 1, 64), (1, 64, 8, 4096), (40, 7, 3, 192), (300, 2, 2, 256), (33, 300, 4, 1024)])
+@pytest.mark.parametrize("T,E,k,K", [(1, 1, 1, 64), (1, 64, 8, 4096), (40, 7, 3, 192), (300, 2, 2, 256), (33, 300, 4, 1024),
+                                     (1030, 1000, 8, 2304), (9000, 3, 2, 1024), (17000, 9, 8, 320), (10300, 37, 8, 2048)])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("drop", [0.0, 0.4])
 def test_dispatch_nvfp4_is_the_quantiser_of_the_sorted_rows(T, E, k, K, dtype, drop):
@@ -140,8 +142,8 @@ def test_dispatch_nvfp4_is_the_quantiser_of_the_sorted_rows(T, E, k, K, dtype, d
     plan = moe.plan(choices(T, E, k, drop, seed=K), E)
     x = _normal((T, K), dtype, 7)
     x[0, :16] = 0                                                   # an all-zero block
-    x[-1, 16:32] *= 1e4                                             # a scale that saturates (or an infinity in fp16: 65504 at most)
-    x = torch.nan_to_num(x)
+    x[-1, 16:32] *= 1e4                                             # a scale that saturates
+    x = torch.nan_to_num(x)                                         # (fp16: 65504 in the place of an infinity)
     a, sfa = moe.dispatch_nvfp4(x, plan)
     codes, scales = F.quantize_nvfp4(x.float())
     src = plan.source.clamp(min=0).long()
