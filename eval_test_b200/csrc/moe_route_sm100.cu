@@ -297,10 +297,16 @@ __device__ __forceinline__ uint32_t same_key(int key, int bits) {
     return same;
 }
 
-// The tokens of a warp of the plan: every warp of every block owns a contiguous run.
-__device__ __forceinline__ int first_token(int T, int warps, long long warp) {
-    const int per = (T + warps - 1) / warps;
-    return (int)min((long long)T, warp * per);
+// Which tokens a block and a warp of it take: contiguous runs, the blocks' of equal length.  A warp takes at least
+// `fewest` tokens (a round of 32 copies, or of the router), so that few tokens do not keep many warps.
+struct TokenRange { int begin, end; };
+__device__ __forceinline__ TokenRange block_tokens(int T, uint32_t blocks, uint32_t block) {
+    const int per = (int)((T + (long long)blocks - 1) / blocks);
+    return {(int)min((long long)T, (long long)block * per), (int)min((long long)T, (long long)(block + 1) * per)};
+}
+__device__ __forceinline__ TokenRange warp_tokens(TokenRange b, int fewest, int warp) {
+    const int per = max((b.end - b.begin + PLAN_WARPS - 1) / PLAN_WARPS, fewest);
+    return {(int)min((long long)b.end, b.begin + (long long)warp * per), (int)min((long long)b.end, b.begin + (long long)(warp + 1) * per)};
 }
 
 // Copies per expert of each block of the spread form (any order: they are only counted).
@@ -310,9 +316,9 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_count_kernel(const PlanA
     __syncthreads();
     pdl_wait();
     pdl_launch();
-    const int begin = first_token(p.T, PLAN_BLOCKS * PLAN_WARPS, (long long)blockIdx.x * PLAN_WARPS) * p.k;
-    const int end = first_token(p.T, PLAN_BLOCKS * PLAN_WARPS, (long long)(blockIdx.x + 1) * PLAN_WARPS) * p.k;
-    for (int i = begin + threadIdx.x; i < end; i += blockDim.x) {
+    const TokenRange b = block_tokens(p.T, gridDim.x, blockIdx.x);
+    const int end = b.end * p.k;
+    for (long long i = (long long)b.begin * p.k + threadIdx.x; i < end; i += blockDim.x) {
         const int e = p.experts[i];
         if ((unsigned)e < (unsigned)p.E) atomicAdd(count + e, 1u);
     }
@@ -339,17 +345,18 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     __shared__ uint32_t live_rows;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = SPREAD ? blockIdx.x : cluster_ctarank(), ctas = SPREAD ? gridDim.x : cluster_size();
-    const long long g = (long long)rank * PLAN_WARPS + warp;
-    const int t0 = first_token(p.T, (int)ctas * PLAN_WARPS, g), t1 = first_token(p.T, (int)ctas * PLAN_WARPS, g + 1);
-    const int begin = t0 * p.k, end = t1 * p.k;         // (T * k < 2^31: checked by the caller)
+    int fewest = (31 + p.k) / p.k;
+    if constexpr (!std::is_void_v<L>) fewest = max(fewest, L::PER_WARP);
+    const TokenRange own_tokens = warp_tokens(block_tokens(p.T, ctas, rank), fewest, warp);
+    const int begin = own_tokens.begin * p.k, end = own_tokens.end * p.k;    // (T * k < 2^31: checked by the caller)
 
     for (int i = threadIdx.x; i < (PLAN_WARPS + 2) * p.E; i += blockDim.x) hist[i] = 0;
     pdl_wait();
     pdl_launch();
     if constexpr (!std::is_void_v<L>) {
-        for (int t = t0; t < t1; t += L::PER_WARP) {
+        for (int t = own_tokens.begin; t < own_tokens.end; t += L::PER_WARP) {
             const int tg = t + lane / L::G;
-            route_token<L>(a, tg < t1 ? tg : a.T, lane % L::G);
+            route_token<L>(a, tg < own_tokens.end ? tg : a.T, lane % L::G);
         }
     }
     __syncthreads();
@@ -371,9 +378,9 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     }
     uint32_t* own = hist + warp * p.E;
     const int bits = 32 - __clz(p.E);                   // keys 0 .. E
-    // (eight loads in flight)
+    // (eight loads in flight; a warp with no more copies than that has its ids still in registers for the second walk)
+    int ids[PLAN_AHEAD];
     for (int i0 = begin; i0 < end; i0 += 32 * PLAN_AHEAD) {
-        int ids[PLAN_AHEAD];
 #pragma unroll
         for (int u = 0; u < PLAN_AHEAD; u++) ids[u] = i0 + 32 * u + lane < end ? p.experts[i0 + 32 * u + lane] : -1;
 #pragma unroll
@@ -426,8 +433,11 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     }
     if (lane == 31) { warp_total[0][warp] = rows_to; warp_total[1][warp] = tiles_to; warp_total[2][warp] = wide_to; }
     __syncthreads();
-    uint32_t row0 = rows_to - count, tile0 = tiles_to - ntiles, wide0 = wide_to - nwide;
-    for (int w = 0; w < warp; w++) { row0 += warp_total[0][w]; tile0 += warp_total[1][w]; wide0 += warp_total[2][w]; }
+    // (PLAN_WARPS = lanes of a warp: the sums of the warps before this one)
+    const bool earlier = lane < warp;
+    const uint32_t row0 = rows_to - count + __reduce_add_sync(0xffffffffu, earlier ? warp_total[0][lane] : 0u);
+    const uint32_t tile0 = tiles_to - ntiles + __reduce_add_sync(0xffffffffu, earlier ? warp_total[1][lane] : 0u);
+    const uint32_t wide0 = wide_to - nwide + __reduce_add_sync(0xffffffffu, earlier ? warp_total[2][lane] : 0u);
     if (threadIdx.x < p.E) {
         base[threadIdx.x] = row0 + before;
         shift[threadIdx.x] = (int)(tile0 * 128u) - (int)row0;
@@ -442,10 +452,11 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     // also: no CTA of a cluster leaves while a peer may still read its counts
     if (SPREAD || ctas == 1) __syncthreads();
     else cluster_sync_all();
+    const bool again = end - begin > 32 * PLAN_AHEAD;
     for (int i0 = begin; i0 < end; i0 += 32 * PLAN_AHEAD) {
-        int ids[PLAN_AHEAD];
 #pragma unroll
-        for (int u = 0; u < PLAN_AHEAD; u++) ids[u] = i0 + 32 * u + lane < end ? p.experts[i0 + 32 * u + lane] : -1;
+        for (int u = 0; u < PLAN_AHEAD; u++)
+            if (again) ids[u] = i0 + 32 * u + lane < end ? p.experts[i0 + 32 * u + lane] : -1;
 #pragma unroll
         for (int u = 0; u < PLAN_AHEAD; u++) {
             if (i0 + 32 * u >= end) break;
@@ -506,11 +517,16 @@ int token_blocks(const RouteArgs& a, int dev) {
 
 template <typename L>
 int launch_route(const RouteArgs& a, const PlanArgs& p, int dev, cudaStream_t st) {
-    // up to 256 tokens the sorting cluster chooses the experts itself, one round of tokens for each of its warps
-    if (a.T <= 256) {
-        int c = 1;
-        while (c < 8 && a.T > PLAN_WARPS * L::PER_WARP * c) c *= 2;
-        return launch_plan<L, false>(p, a, c, st);
+    // few tokens: the sorting cluster chooses the experts itself (one launch against two: 1 x 128 bf16 6.4 / 6.9 us, 128 x
+    // 128 7.3 / 8.5, 512 x 64 7.7 / 8.7; not where a lane holds sixteen unpacked entries, which the 64 registers of its 1024
+    // threads do not: 32 x 256 fp32 12.0 / 8.4).  The choice is bound by instruction issue, so the CTAs take four warps'
+    // tokens each as long as there are CTAs
+    if constexpr (L::PACKED ? L::NV <= 16 : L::NV <= 8) {
+        if (a.T <= 512) {
+            int c = 1;
+            while (c < 8 && a.T > 4 * L::PER_WARP * c) c *= 2;
+            return launch_plan<L, false>(p, a, c, st);
+        }
     }
     const int rc = launch_dependent(route_kernel<L>, token_blocks<L>(a, dev), 256, 0, 0, st, a);
     return rc ? rc : plan_choices(p, st);
