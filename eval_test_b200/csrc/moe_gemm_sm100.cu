@@ -46,6 +46,10 @@
 #include "quant_block.cuh"
 
 namespace nvfp4 {
+
+// Status word of a device if an earlier call has already created it, else nullptr (defined in common.cu).
+int* status_word_if_allocated(int dev);
+
 namespace {
 
 constexpr int XM = 128;                              // weight rows of a CTA and tile
@@ -429,6 +433,18 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     }
 }
 
+// The device's status word.  Its first use allocates it, which a capture in global mode forbids the thread that captures:
+// the mode is relaxed for that moment (the allocation belongs to no graph).
+int* status_word_anywhere(int dev) {
+    int* word = status_word_if_allocated(dev);
+    if (word) return word;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    word = status_word(dev);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    return word;
+}
+
 // Tiles of `rows` rows that R copies over E experts can fill at most: every expert that has rows has at most one tile
 // that is not full.
 long most_tiles(int R, int E, int rows) {
@@ -498,7 +514,7 @@ int expert_product(const void* a, const void* sfa_sw, const void* b, const void*
     if (rc) return rc;
     if (!DUAL) { maps.b2 = maps.b; maps.sb2 = maps.sb; }
     const ExpertParams p{(const int*)offsets, (const int*)tiles, (const int*)wide, (const float*)alphas, (uint8_t*)c, (uint8_t*)sfc,
-                         R, E, N, K, alpha, status_word(dev), wait_budget_ns()};
+                         R, E, N, K, alpha, status_word_anywhere(dev), wait_budget_ns()};
     cudaStream_t st = (cudaStream_t)stream;
     // few rows per expert on average (64 experts, K = 7168, experts liked unequally, NT = 128 against 256): 32 rows 161
     // against 169 us, 64: 172 / 175, 96: 188 / 187, 128: 217 / 204; DUAL 32: 159 / 172, 96: 182 / 200, 128: 213 / 208

@@ -321,9 +321,6 @@ __global__ void __launch_bounds__(256) gather_scales_kernel(const uint8_t* __res
     }
 }
 
-// Vectors per lane: one as long as that gives every SM a few warps, else U.
-bool spread(long long T, int row_vecs, int dev) { return T * ((row_vecs + 31) / 32) <= 16ll * sm_count(dev); }
-
 // Blocks of a grid-stride launch over n threads: at most eight resident blocks per SM.
 int grid_for(long long n, int dev) {
     long long blocks = (n + 255) / 256;
@@ -385,7 +382,10 @@ extern "C" int nvfp4_moe_dispatch(const void* x, int kind, long long ld, const v
         return launch_dependent(dispatch_kernel<B, U>, grid_for(32 * warps, dev), 256, 0, 0, st, (const uint8_t*)x, ld * size, xs, row_vecs, p);
     };
     auto go_bytes = [&](auto bytes) {
-        return spread(T, row_vecs, dev) ? go(bytes, std::integral_constant<int, 1>()) : go(bytes, std::integral_constant<int, 4>());
+        // one vector per lane while that fills the SMs at most once, else four (bf16, one against four: 8 x 8 x 7168 2.0 /
+        // 3.5 us, 256 x 8 x 4096 3.8 / 4.1, 16384 x 8 x 4096 220 / 204)
+        const bool one = (long long)T * ((row_vecs + 31) / 32) <= 32ll * sm_count(dev);
+        return one ? go(bytes, std::integral_constant<int, 1>()) : go(bytes, std::integral_constant<int, 4>());
     };
     switch (vec) {
         case 16: return go_bytes(std::integral_constant<int, 16>());
@@ -427,7 +427,8 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
             };
             using std::integral_constant;
             auto go_width = [&](auto vn) {
-                if (spread(T, row_vecs, dev)) return go(vn, integral_constant<int, 8>(), integral_constant<int, 1>());
+                // as many loads in flight for few choices as for eight (bf16, 512 x 2 x 2048: 2.0 us, 3.2 with one vector
+                // of eight rows, 128 x 4 x 4096: 1.9 / 2.4)
                 // (of two rows, as many vectors as eight rows have: 4096 x 2 x 2048 fp32 17.3 us with four against 19.0 with two)
                 if (k <= 2) return go(vn, integral_constant<int, 2>(), integral_constant<int, VN == 4 ? 4 : 2>());
                 if (k <= 4) return go(vn, integral_constant<int, 4>(), integral_constant<int, 2>());

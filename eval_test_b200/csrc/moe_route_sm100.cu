@@ -265,12 +265,15 @@ struct PlanArgs {
     int* rows;                 // [T][k] sorted row of a copy, -1: none
     int* slots;                // [T][k] the row counted with every expert padded to whole tiles, -1: none
     int* source;               // [T*k] copy of a sorted row, -1 behind the last
-    uint32_t* counts;          // [PLAN_BLOCKS][E] copies of a block: the spread form only
+    uint32_t* counts;          // [blocks][E] copies of a block: the spread form only
     int T, E, k;
 };
 
 constexpr int PLAN_WARPS = 32;
-constexpr int PLAN_BLOCKS = 128;   // of the spread form
+// Blocks of the spread form: every block sums the counts of all, so the more experts there are, the fewer blocks (131072
+// copies: 64 experts 8.6 us with 128 blocks; 256 experts 15.3 us with 128, 12.8 us with 32; 1024 experts 40.5 us with
+// 128, 22.8 us with 16).
+__host__ __device__ constexpr int plan_blocks(int E) { return E <= 64 ? 128 : E >= 512 ? 16 : 8192 / E; }
 constexpr long long PLAN_CLUSTER_MOST = 16384;   // copies that are sorted by one cluster
 constexpr int PLAN_AHEAD = 8;      // rounds of 32 copies whose ids a warp has in flight
 
@@ -331,9 +334,9 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32) plan_count_kernel(const PlanA
 // it is that of the copies, and nothing is left behind between calls.
 //   one cluster (SPREAD = false): the blocks exchange their counts through distributed shared memory.  One launch, no
 //     scratch; L: the warps choose their tokens' experts first, in that layout (few tokens: router and plan in one);
-//   spread: PLAN_BLOCKS blocks on as many SMs, whose counts plan_count_kernel has left in memory.
-// 131072 copies, 64 experts: 25.8 us in a cluster of 8 (what bounds it is the scattered stores and the votes of eight
-// SMs), 13 us spread over 128 blocks, the counting included; up to 16384 copies the one launch is faster.
+//   spread: plan_blocks(E) blocks on as many SMs, whose counts plan_count_kernel has left in memory.
+// 131072 copies, 64 experts: 23.9 us in a cluster of 8 (what bounds it is the scattered stores and the votes of eight
+// SMs), 8.6 us spread over 128 blocks, the counting included; 16384 copies: 6.3 and 7.1 us.
 template <typename L, bool SPREAD>
 __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs p, const RouteArgs a) {
     extern __shared__ uint32_t plan_smem[];
@@ -495,17 +498,15 @@ int launch_plan(const PlanArgs& p, const RouteArgs& a, int ctas, cudaStream_t st
     return launch_dependent(plan_kernel<L, SPREAD>, ctas, PLAN_WARPS * 32, (size_t)(PLAN_WARPS + 3) * p.E * 4, SPREAD ? 0 : ctas, st, p, a);
 }
 
-// The plan of choices that are in memory.  In a cluster: one CTA for up to 1024 copies, then up to the eight that every
-// device can place.
+// The plan of choices that are in memory.  In a cluster: one CTA or the eight that every device can place (64 experts, one
+// against eight: 512 copies 3.1 / 3.7 us, 1024 4.0 / 3.7, 8192 12.7 / 5.0).
 int plan_choices(const PlanArgs& p, cudaStream_t st) {
     const long long copies = (long long)p.T * p.k;
     if (copies > PLAN_CLUSTER_MOST) {
-        int rc = launch_dependent(plan_count_kernel, PLAN_BLOCKS, PLAN_WARPS * 32, 0, 0, st, p);
-        return rc ? rc : launch_plan<void, true>(p, RouteArgs{}, PLAN_BLOCKS, st);
+        int rc = launch_dependent(plan_count_kernel, plan_blocks(p.E), PLAN_WARPS * 32, 0, 0, st, p);
+        return rc ? rc : launch_plan<void, true>(p, RouteArgs{}, plan_blocks(p.E), st);
     }
-    int c = 1;
-    while (c < 8 && copies > 1024ll * c) c *= 2;
-    return launch_plan<void, false>(p, RouteArgs{}, c, st);
+    return launch_plan<void, false>(p, RouteArgs{}, copies <= 512 ? 1 : 8, st);
 }
 
 // Blocks of eight warps for `a.T` tokens, at most eight on an SM.
@@ -563,7 +564,7 @@ int check_route(int kind, long long ld, int T, int E, int k) {
 using namespace nvfp4;
 
 extern "C" long long nvfp4_moe_plan_scratch(int T, int E, int k) {
-    return T > 0 && E > 0 && k > 0 && (long long)T * k > PLAN_CLUSTER_MOST ? 4ll * PLAN_BLOCKS * E : 0;
+    return T > 0 && E > 0 && k > 0 && (long long)T * k > PLAN_CLUSTER_MOST ? 4ll * plan_blocks(E) * E : 0;
 }
 
 extern "C" int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* offsets, void* tiles, void* wide_tiles, void* rows,

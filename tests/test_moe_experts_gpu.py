@@ -6,10 +6,11 @@ from _moe import choices, dequant
 
 pytestmark = pytest.mark.gpu
 BF16 = torch.bfloat16
-# T, E, k, N, K, share of dropped choices: one row; short last boxes; several tiles of one expert; every tile width
+# T, E, k, N, K, share of dropped choices: one row; short last boxes; several tiles of one expert; both tile widths, with
+# more tiles than the machine takes at once
 SIZES = [(1, 4, 2, 128, 256, 0.0), (5, 3, 1, 256, 512, 0.0), (40, 5, 3, 640, 768, 0.3), (300, 2, 2, 384, 256, 0.1),
          (129, 1, 1, 128, 512, 0.0), (700, 9, 1, 256, 1024, 0.0), (256, 64, 2, 1024, 512, 0.05), (2, 300, 2, 128, 256, 0.0),
-         (1, 64, 8, 2048, 4096, 0.0), (1600, 4, 2, 1024, 512, 0.02)]
+         (1, 64, 8, 2048, 4096, 0.0), (1600, 4, 2, 1024, 512, 0.02), (3000, 8, 2, 2176, 512, 0.0)]
 
 
 def _operands(T, E, k, N, K, drop, weights=1, seed=0):
@@ -207,6 +208,70 @@ def test_layer_in_a_graph_follows_its_inputs():
         for T, x, logits, mask, graph, out in made:
             assert torch.equal(out, _layer(moe, x, logits, k, ops, mask))
     _ok_status()
+
+
+def test_first_calls_of_a_process_can_be_captured():
+    """Nothing has to have run before: what the first calls set up (the status word, kernel attributes) is no part of
+    the graph and does not break the capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = """
+import sys; sys.path.insert(0, 'tests')
+import torch
+from test_moe_experts_gpu import _layer, _layer_weights, BF16
+from eval_test_b200 import moe, _lib
+ops = _layer_weights(6, 256, 512)
+x, logits = torch.randn((40, 512), device='cuda').to(BF16), torch.randn((40, 6), device='cuda')
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = _layer(moe, x, logits, 2, ops)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, _layer(moe, x, logits, 2, ops)) and out.any()
+torch.cuda.synchronize()
+assert _lib.device_status(0) == 0
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=str(Path(__file__).resolve().parent.parent), capture_output=True, text=True,
+                          timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_outputs_behind_two_to_the_31_elements():
+    """Rows whose offsets pass 32 bits, in elements and in bytes."""
+    from eval_test_b200 import moe, quantize
+    T, E, k, N, K = 34000, 4, 8, 8192, 256                          # 272000 rows of 8192: 2.2e9 outputs
+    g = torch.Generator(device="cuda").manual_seed(4)
+    ids = torch.randint(0, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    plan = moe.plan(ids, E)
+    x = torch.randn((T, K), generator=g, device="cuda").to(BF16)
+    b, sf, sf_p = quantize.quantize_operand(torch.randn((E, N, K), generator=g, device="cuda"))
+    a, sfa = moe.dispatch_nvfp4(x, plan)
+    y = moe.expert_gemm(a, sfa, b, sf_p, plan)
+    _ok_status()
+    from eval_test_b200 import formats as F
+    codes, scales = F.quantize_nvfp4(x.float())
+    a64 = dequant(codes, scales.view(torch.float8_e4m3fn))
+    w64 = dequant(b.view(torch.uint8).permute(2, 0, 1), sf.permute(2, 0, 1))
+    rows = torch.tensor([0, 131071, 262143, 262144, 262145, T * k - 1], device="cuda")
+    copies = plan.source[rows].long()
+    e = ids.reshape(-1)[copies].long()
+    exact = torch.einsum("rk,rnk->rn", a64[copies // k], w64[e])
+    size = torch.einsum("rk,rnk->rn", a64[copies // k].abs(), w64[e].abs())
+    room = (K / 64 + 4) * 2.0 ** -23 * size + 2.0 ** -11 * exact.abs() * (1 + 2 ** -8) + 2.0 ** -25
+    assert torch.all((y[rows].double() - exact).abs() <= room)
+    # the same buffer back, and out again
+    w = torch.rand((T, k), generator=g, device="cuda")
+    out = moe.combine(y, plan, w, dtype=BF16)
+    t = torch.tensor([0, 16000, T - 1], device="cuda")
+    parts = w[t].double()[..., None] * y[plan.rows[t].long()].double()
+    assert torch.all((out[t].double() - parts.sum(1)).abs() <= k * 2.0 ** -24 * parts.abs().sum(1) + 2.0 ** -8 * parts.sum(1).abs() * (1 + 2 ** -10))
+    dy, dw = moe.combine_backward(out, y, plan, w)
+    want = (w.reshape(-1)[copies][:, None] * out[copies // k].float()).half()
+    assert torch.equal(dy[rows], want)
+    xs = moe.dispatch(out, plan)
+    assert torch.equal(xs[rows], out[copies // k])
 
 
 def test_layer_on_two_streams_at_once():
