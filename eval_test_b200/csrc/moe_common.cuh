@@ -33,6 +33,13 @@ template <> struct Bits<8> { using type = uint2; };
 template <> struct Bits<4> { using type = uint32_t; };
 template <> struct Bits<2> { using type = uint16_t; };
 
+// 16 bytes that are read once (no line of L1 is kept for them).  A volatile asm stays behind the pdl_wait() before it.
+__device__ __forceinline__ uint4 load_once(const void* p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
 // N consecutive elements (2, 4, 8, 16 or 32 bytes) kept as they lie in memory, two 16-bit elements to a register, until
 // they are looked at: as arrays of 16-bit values the compiler gave each element a register of its own, and the kernels
 // with eight vectors in flight fell to a quarter of the SM's threads.  Aligned to its size, at most 16 bytes.
@@ -41,11 +48,13 @@ struct Vec {
     static constexpr int BYTES = N * (int)sizeof(T), WORDS = (BYTES + 3) / 4;
     uint32_t w[WORDS];
 
+    template <bool ONCE = false>
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (BYTES >= 16) {
 #pragma unroll
             for (int i = 0; i < WORDS / 4; i++) {
-                const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+                const uint4* at = reinterpret_cast<const uint4*>(p) + i;
+                const uint4 v = ONCE ? load_once(at) : *at;
                 w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
             }
         } else if constexpr (BYTES == 8) {

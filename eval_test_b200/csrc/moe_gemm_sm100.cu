@@ -245,9 +245,9 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
 
     int* tables = reinterpret_cast<int*>(smem_raw + (smem0 - smem_u32(smem_raw)) + STAGES * Stage::BYTES + x_epilogue_warps(NT) * X_TURN_BYTES);
     for (int i = threadIdx.x; i <= p.E; i += blockDim.x) {
-        tables[i] = __ldg(p.offsets + i);
-        tables[p.E + 1 + i] = __ldg(p.tiles + i);
-        tables[2 * (p.E + 1) + i] = __ldg((NT == 128 ? p.tiles : p.wide) + i);
+        tables[i] = p.offsets[i];
+        tables[p.E + 1 + i] = p.tiles[i];
+        tables[2 * (p.E + 1) + i] = (NT == 128 ? p.tiles : p.wide)[i];
     }
     __syncthreads();
     ExpertTables where{tables, tables + p.E + 1, tables + 2 * (p.E + 1), (p.N + 2 * XM - 1) / (2 * XM), 0};
@@ -366,7 +366,7 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         for (int t = pair; alive && t < total_tiles; t += npairs) {
             const ExpertTile ti = where.locate<NT>(t, rank);
             const int chunks = (ti.n + 31) / 32;         // with tokens in them
-            const float alpha = p.alphas ? p.alpha * __ldg(p.alphas + ti.e) : p.alpha;
+            const float alpha = p.alphas ? p.alpha * p.alphas[ti.e] : p.alpha;
             const bool block_exists = ti.w < p.N / XM;
             uint32_t held[DUAL ? 2 : 1][32];             // x, then silu(x) until y is there
             uint32_t out[2][16];                         // fp16 results, two tokens to a register

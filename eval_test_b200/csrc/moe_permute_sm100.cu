@@ -64,8 +64,8 @@ struct Pieces {
         next_w = 0.f;
         if (at < n && lane < k) {
             const size_t copy = (size_t)next_t * k + lane;
-            next_row = __ldg(rows + copy);
-            if (WEIGHTED) next_w = __ldg(weights + copy);
+            next_row = rows[copy];
+            if (WEIGHTED) next_w = weights[copy];
         }
     }
     __device__ __forceinline__ void locate() {
@@ -81,8 +81,7 @@ struct Pieces {
 
 // One load of a token's vector, k stores.
 template <int BYTES, int U>
-__global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* __restrict__ x, long long ld, void* __restrict__ xs,
-                                                       int row_vecs, const PermuteArgs p) {
+__global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* x, long long ld, void* xs, int row_vecs, const PermuteArgs p) {
     using V = typename Bits<BYTES>::type;
     pdl_wait();
     pdl_launch();
@@ -92,7 +91,7 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* __restrict
         V v[U];
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (w.c + 32 * u < row_vecs) v[u] = __ldg(src + w.c + 32 * u);
+            if (w.c + 32 * u < row_vecs) v[u] = src[w.c + 32 * u];
         for (int j = 0; j < p.k; j++) {
             const int row = __shfl_sync(0xffffffffu, w.row, j);
             if (row < 0) continue;
@@ -105,10 +104,12 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* __restrict
     zero_tail(out, row_vecs, p);
 }
 
-// KU rows' loads of U vectors each are in flight at a time.  `pitch`: bytes between rows of y.
+// KU rows' loads of U vectors each are in flight at a time.  `pitch`: bytes between rows of y.  (Loads past L1 are faster
+// for few rows, 4096 x 2 x 2048 fp32 14.7 against 19.3 us, 8192 x 4 x 4096 bf16 54.6 / 56.3, and slower for eight, whose
+// loads the compiler then cannot place among the sums: 16384 x 8 x 4096 197 / 180.)
 template <typename TI, typename TO, int VN, int KU, int U, bool WEIGHTED>
-__global__ void __launch_bounds__(256, U >= 2 ? 3 : 4) combine_kernel(const TI* __restrict__ y, unsigned pitch, const float* __restrict__ weights,
-                                                         TO* __restrict__ out, int row_vecs, const PermuteArgs p) {
+__global__ void __launch_bounds__(256, U >= 2 ? 3 : 4) combine_kernel(const TI* y, unsigned pitch, const float* weights, TO* out,
+                                                                      int row_vecs, const PermuteArgs p) {
     pdl_wait();
     pdl_launch();
     for (Pieces<U, WEIGHTED> w(p, weights, row_vecs); w.more(); w.next()) {
@@ -122,7 +123,7 @@ __global__ void __launch_bounds__(256, U >= 2 ? 3 : 4) combine_kernel(const TI* 
                 const TI* src = reinterpret_cast<const TI*>(at + (unsigned long long)(unsigned)row * pitch);
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    if (row >= 0 && w.c + 32 * u < row_vecs) v[j][u].load(src + 32 * u * VN);
+                    if (row >= 0 && w.c + 32 * u < row_vecs) v[j][u].template load<(KU < 8)>(src + 32 * u * VN);
             }
 #pragma unroll
             for (int j = 0; j < KU; j++) {
@@ -147,9 +148,8 @@ __global__ void __launch_bounds__(256, U >= 2 ? 3 : 4) combine_kernel(const TI* 
 // rows; their dot products stay in registers and are summed over the group at the end, in an order that depends on the
 // sizes alone.  `pitch`: bytes between rows of y.
 template <typename TI, typename TO, int VN, int GROUP, int KU, int U>
-__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* __restrict__ dout, long long ldo, const TI* __restrict__ y,
-                                                                  unsigned pitch, const float* __restrict__ weights,
-                                                                  TI* __restrict__ dy, float* __restrict__ dw, int row_vecs,
+__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* dout, long long ldo, const TI* y, unsigned pitch,
+                                                                  const float* weights, TI* dy, float* dw, int row_vecs,
                                                                   const PermuteArgs p) {
     __shared__ float part[8][KU];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* __re
             float w[KU], acc[KU];
 #pragma unroll
             for (int j = 0; j < KU; j++) {
-                row[j] = j0 + j < p.k ? __ldg(p.rows + t * p.k + j0 + j) : -1;
-                w[j] = row[j] >= 0 ? __ldg(weights + t * p.k + j0 + j) : 0.f;
+                row[j] = j0 + j < p.k ? p.rows[t * p.k + j0 + j] : -1;
+                w[j] = row[j] >= 0 ? weights[t * p.k + j0 + j] : 0.f;
                 acc[j] = 0.f;
             }
             for (int c = in_group; c < row_vecs; c += GROUP * U) {
@@ -238,22 +238,19 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* __re
 // gather_scales_kernel makes whole atoms: 4-byte stores 512 bytes apart took as long as everything else together
 // (16384 tokens x 8 x 4096: 130 us, 90 us with the table).
 template <int KIND, bool TABLE>
-__global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* __restrict__ x, long long ld, const int* __restrict__ slots,
-                                                             uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
-                                                             const PermuteArgs p) {
+__global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* x, long long ld, const int* slots, uint8_t* codes,
+                                                             uint8_t* scales, const PermuteArgs p) {
     using T = typename ElemOf<KIND>::type;
     pdl_wait();
     pdl_launch();
-    const int units = p.H / 32;
-    const int lane = threadIdx.x & 31;
-    const long long n = (long long)p.T * units, step = (long long)gridDim.x * blockDim.x;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i - lane < n; i += step) {
+    const unsigned units = p.H / 32, lane = threadIdx.x & 31;
+    const unsigned n = (unsigned)p.T * units, step = gridDim.x * blockDim.x;    // (fewer than 2^31: checked by the caller)
+    for (unsigned i = blockIdx.x * blockDim.x + threadIdx.x; i - lane < n; i += step) {
         const bool in = i < n;
-        const long long t = in ? i / units : 0;
-        const int c = in ? (int)(i - t * units) : 0;
+        const unsigned t = in ? i / units : 0, c = in ? i - t * units : 0;
         float xs[32];
         constexpr int VN = 16 / (int)sizeof(T);
-        const T* src = reinterpret_cast<const T*>(x) + t * ld + (long long)c * 32;
+        const T* src = reinterpret_cast<const T*>(x) + t * ld + (size_t)c * 32;
 #pragma unroll
         for (int v = 0; v < 32 / VN; v++) {
             Vec<T, VN> a;
@@ -270,16 +267,24 @@ __global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* __restr
             s |= __shfl_down_sync(0xffffffffu, s, 1) << 16;   // (n is even: the two lanes of a group are in range together)
         }
         if (!in) continue;
-        const int* rows = p.rows + t * p.k;
-        uint8_t* dst = codes + (long long)c * 16;
-        for (int j = 0; j < p.k; j++) {
-            const int row = __ldg(rows + j);
-            if (row < 0) continue;
-            *reinterpret_cast<uint4*>(dst + (long long)row * units * 16) = w;
-            if (!TABLE && (lane & 1) == 0) {
-                const int slot = __ldg(slots + t * p.k + j);
-                const long long atom = (long long)(slot >> 7) * (units / 2) + c / 2;
-                *reinterpret_cast<uint32_t*>(scales + atom * 512 + (slot & 31) * 16 + ((slot & 127) >> 5) * 4) = s;
+        const int* rows = p.rows + (size_t)t * p.k;
+        const int* at = slots + (size_t)t * p.k;
+        uint8_t* dst = codes + (size_t)c * 16;
+        for (int j0 = 0; j0 < p.k; j0 += 4) {
+            int row[4], slot[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                row[j] = j0 + j < p.k ? rows[j0 + j] : -1;
+                slot[j] = !TABLE && j0 + j < p.k ? at[j0 + j] : 0;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (row[j] < 0) continue;
+                *reinterpret_cast<uint4*>(dst + (long long)row[j] * units * 16) = w;
+                if (!TABLE && (lane & 1) == 0) {
+                    const long long atom = (long long)(slot[j] >> 7) * (units / 2) + c / 2;
+                    *reinterpret_cast<uint32_t*>(scales + atom * 512 + (slot[j] & 31) * 16 + ((slot[j] & 127) >> 5) * 4) = s;
+                }
             }
         }
     }
@@ -288,31 +293,30 @@ __global__ void __launch_bounds__(256) dispatch_quant_kernel(const void* __restr
 
 // The scale atoms of one 128-row tile from the tokens' scale rows: a warp makes four atoms (256 elements of K) at a time,
 // lane i the 16 bytes of the rows i, i + 32, i + 64, i + 96 in each.  Rows that do not exist get zeros.
-__global__ void __launch_bounds__(256) gather_scales_kernel(const uint8_t* __restrict__ table, const int* __restrict__ source,
-                                                            const int* __restrict__ offsets, const int* __restrict__ tiles,
-                                                            uint8_t* __restrict__ sf_sw, int E, int k, int K) {
+__global__ void __launch_bounds__(256) gather_scales_kernel(const uint8_t* table, const int* source, const int* offsets,
+                                                            const int* tiles, uint8_t* sf_sw, int E, int k, int K) {
     __shared__ int expert;
     pdl_wait();
     pdl_launch();
     const int tile = blockIdx.x;
-    if (tile >= __ldg(tiles + E)) return;
+    if (tile >= tiles[E]) return;
     for (int e = threadIdx.x; e < E; e += blockDim.x)
-        if (__ldg(tiles + e) <= tile && tile < __ldg(tiles + e + 1)) expert = e;
+        if (tiles[e] <= tile && tile < tiles[e + 1]) expert = e;
     __syncthreads();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int row0 = __ldg(offsets + expert) + (tile - __ldg(tiles + expert)) * 128, end = __ldg(offsets + expert + 1);
+    const int row0 = offsets[expert] + (tile - tiles[expert]) * 128, end = offsets[expert + 1];
     long long token[4];
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         const int row = row0 + q * 32 + lane;
-        token[q] = row < end ? __ldg(source + row) / k : -1;
+        token[q] = row < end ? source[row] / k : -1;
     }
     const int chunks = K / 256;
     for (int c = blockIdx.y * 8 + warp; c < chunks; c += gridDim.y * 8) {
         uint4 w[4];
 #pragma unroll
         for (int q = 0; q < 4; q++)
-            w[q] = token[q] >= 0 ? __ldg(reinterpret_cast<const uint4*>(table + token[q] * (K / 16)) + c) : make_uint4(0u, 0u, 0u, 0u);
+            w[q] = token[q] >= 0 ? reinterpret_cast<const uint4*>(table + token[q] * (K / 16))[c] : make_uint4(0u, 0u, 0u, 0u);
         uint4* dst = reinterpret_cast<uint4*>(sf_sw + ((long long)tile * (K / 64) + c * 4) * 512) + lane;
         dst[0] = make_uint4(w[0].x, w[1].x, w[2].x, w[3].x);
         dst[32] = make_uint4(w[0].y, w[1].y, w[2].y, w[3].y);
@@ -504,6 +508,7 @@ extern "C" int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, c
     if (rc) return rc;
     if (E <= 0) return NVFP4_ERR_SHAPE;
     if (K % 64 != 0) return NVFP4_ERR_K_MULTIPLE;
+    if ((long long)T * (K / 32) >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
     const bool table = nvfp4_moe_dispatch_scratch(T, k, K) > 0;
     if (table && !scratch) return NVFP4_ERR_NULL;
     if (((uintptr_t)x & 15) || ld * elem_bytes(kind) % 16 || ((uintptr_t)packed & 15) || ((uintptr_t)sf_sw & 15) ||

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs a) {
 
 // G lanes, one token.  The chosen experts' terms are handed round by shuffles, so every entry is written once.
 template <typename L>
-__global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a, const float* __restrict__ dw, void* dlogits) {
+__global__ void __launch_bounds__(256) route_backward_kernel(const RouteArgs a, const float* dw, void* dlogits) {
     using T = typename L::T;
     constexpr int G = L::G, NV = L::NV;
     pdl_wait();

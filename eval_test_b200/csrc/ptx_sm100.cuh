@@ -86,7 +86,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint64_
 // Programmatic dependent launch.  A kernel launched with that attribute may start while the kernel before it in the
 // stream still runs: pdl_wait() returns when that kernel has completed and its memory is visible, pdl_launch() says that
 // the next one may start.  Both do nothing in a kernel launched without the attribute.  Every kernel that is launched
-// with it waits before it touches global memory, so the kernels of a stream still take effect in order.
+// with it waits before it touches global memory, so the kernels of a stream still take effect in order.  Such a kernel
+// reads through plain pointers only: a load that the compiler may take for invariant (__ldg, a const __restrict__
+// parameter) could be moved in front of the wait.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
