@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* x, long lo
 // for few rows, 4096 x 2 x 2048 fp32 14.7 against 19.3 us, 8192 x 4 x 4096 bf16 54.6 / 56.3, and slower for eight, whose
 // loads the compiler then cannot place among the sums: 16384 x 8 x 4096 197 / 180.)
 template <typename TI, typename TO, int VN, int KU, int U, bool WEIGHTED>
-__global__ void __launch_bounds__(256, U >= 2 ? 3 : 4) combine_kernel(const TI* y, unsigned pitch, const float* weights, TO* out,
+__global__ void __launch_bounds__(256, U >= 2 && VN > 1 ? 3 : 4) combine_kernel(const TI* y, unsigned pitch, const float* weights, TO* out,
                                                                       int row_vecs, const PermuteArgs p) {
     pdl_wait();
     pdl_launch();
@@ -415,11 +415,12 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
         return by_type(out_kind, [&](auto to) {
             using TI = decltype(ti);
             using TO = decltype(to);
-            // vectors of 16 input bytes where both sides are aligned to theirs
+            // vectors of 16 input bytes where both sides are aligned to theirs, else 16-bit elements in pairs, else one by one
             constexpr int VN = 16 / sizeof(TI);
             constexpr unsigned long long O = VN * sizeof(TO) < 16 ? VN * sizeof(TO) : 16;
             const bool wide = H % VN == 0 && ld % VN == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)out % O == 0;
-            const int row_vecs = wide ? H / VN : H;
+            const bool pair = sizeof(TI) == 2 && !wide && H % 2 == 0 && ld % 2 == 0 && (uintptr_t)y % 4 == 0 && (uintptr_t)out % (2 * sizeof(TO)) == 0;
+            const int row_vecs = wide ? H / VN : pair ? H / 2 : H;
             auto go = [&](auto vn, auto ku, auto u) {
                 constexpr int N = decltype(vn)::value, KU = decltype(ku)::value, U = decltype(u)::value;
                 const long long warps = (long long)T * ((row_vecs + 32 * U - 1) / (32 * U));
@@ -432,12 +433,17 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
             using std::integral_constant;
             auto go_width = [&](auto vn) {
                 // as many loads in flight for few choices as for eight (bf16, 512 x 2 x 2048: 2.0 us, 3.2 with one vector
-                // of eight rows, 128 x 4 x 4096: 1.9 / 2.4)
-                // (of two rows, as many vectors as eight rows have: 4096 x 2 x 2048 fp32 17.3 us with four against 19.0 with two)
-                if (k <= 2) return go(vn, integral_constant<int, 2>(), integral_constant<int, VN == 4 ? 4 : 2>());
+                // of eight rows, 128 x 4 x 4096: 1.9 / 2.4; of two rows, fp32 4096 x 2 x 2048 17.3 us with four vectors,
+                // 19.0 with two), and more where a vector is one or two elements (8192 x 8 x 4002 fp16, one, two, four
+                // vectors of eight rows: 192, 159, 297 us; 4001 wide 332, 275, 314)
+                constexpr int N = decltype(vn)::value;
+                if (k <= 2) return go(vn, integral_constant<int, 2>(), integral_constant<int, N == 8 ? 2 : 4>());
                 if (k <= 4) return go(vn, integral_constant<int, 4>(), integral_constant<int, 2>());
-                return go(vn, integral_constant<int, 8>(), integral_constant<int, 1>());
+                return go(vn, integral_constant<int, 8>(), integral_constant<int, N <= 2 ? 2 : 1>());
             };
+            if constexpr (sizeof(TI) == 2) {
+                if (pair) return go_width(integral_constant<int, 2>());
+            }
             return wide ? go_width(integral_constant<int, VN>()) : go_width(integral_constant<int, 1>());
         });
     });
@@ -467,7 +473,9 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
             constexpr unsigned long long O = VN * sizeof(TO) < 16 ? VN * sizeof(TO) : 16;
             const bool wide = H % VN == 0 && ld % VN == 0 && ldo % VN == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)dy % 16 == 0 &&
                               (uintptr_t)dout % O == 0;
-            const int row_vecs = wide ? H / VN : H;
+            const bool pair = sizeof(TI) == 2 && !wide && H % 2 == 0 && ld % 2 == 0 && ldo % 2 == 0 && (uintptr_t)y % 4 == 0 &&
+                              (uintptr_t)dy % 4 == 0 && (uintptr_t)dout % (2 * sizeof(TO)) == 0;
+            const int row_vecs = wide ? H / VN : pair ? H / 2 : H;
             // a warp per token where its lanes take at most four vectors each, and for few choices where there are tokens
             // enough for that (bf16, 4096 wide, a warp against a block: 16384 x 1 65 against 86 us, 8192 x 4 98 / 105; with
             // eight rows in registers a warp's loads no longer cover its stores: 16384 x 8 372 / 351)
@@ -481,13 +489,17 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
             };
             using std::integral_constant;
             auto go_group = [&](auto vn, auto group) {
-                if (k <= 2) return go(vn, group, integral_constant<int, 2>(), integral_constant<int, 2>());
-                if (k <= 4) return go(vn, group, integral_constant<int, 4>(), integral_constant<int, 2>());
-                return go(vn, group, integral_constant<int, 8>(), integral_constant<int, 1>());
+                constexpr int N = decltype(vn)::value;
+                if (k <= 2) return go(vn, group, integral_constant<int, 2>(), integral_constant<int, N <= 2 ? 8 : 2>());
+                if (k <= 4) return go(vn, group, integral_constant<int, 4>(), integral_constant<int, N <= 2 ? 4 : 2>());
+                return go(vn, group, integral_constant<int, 8>(), integral_constant<int, N <= 2 ? 2 : 1>());
             };
             auto go_width = [&](auto vn) {
                 return warp ? go_group(vn, integral_constant<int, 32>()) : go_group(vn, integral_constant<int, 256>());
             };
+            if constexpr (sizeof(TI) == 2) {
+                if (pair) return go_width(integral_constant<int, 2>());
+            }
             return wide ? go_width(integral_constant<int, VN>()) : go_width(integral_constant<int, 1>());
         });
     });
