@@ -10,7 +10,8 @@ BF16 = torch.bfloat16
 # more tiles than the machine takes at once
 SIZES = [(1, 4, 2, 128, 256, 0.0), (5, 3, 1, 256, 512, 0.0), (40, 5, 3, 640, 768, 0.3), (300, 2, 2, 384, 256, 0.1),
          (129, 1, 1, 128, 512, 0.0), (700, 9, 1, 256, 1024, 0.0), (256, 64, 2, 1024, 512, 0.05), (2, 300, 2, 128, 256, 0.0),
-         (1, 64, 8, 2048, 4096, 0.0), (1600, 4, 2, 1024, 512, 0.02), (3000, 8, 2, 2176, 512, 0.0)]
+         (1, 64, 8, 2048, 4096, 0.0), (1600, 4, 2, 1024, 512, 0.02), (3000, 8, 2, 2176, 512, 0.0),
+         (40, 1024, 3, 128, 256, 0.1)]
 
 
 def _operands(T, E, k, N, K, drop, weights=1, seed=0):
@@ -189,7 +190,7 @@ def test_layer_in_a_graph_follows_its_inputs():
     ops = _layer_weights(E, N, K)
     g = torch.Generator(device="cuda").manual_seed(5)
     made = []
-    for T in (1, 150):
+    for T in (1, 150, 6000):                                        # the last: a sort of several launches
         x, logits = torch.zeros((T, K), device="cuda", dtype=BF16), torch.zeros((T, E), device="cuda")
         mask = torch.ones((T,), dtype=torch.bool, device="cuda")
         _layer(moe, x, logits, k, ops, mask)

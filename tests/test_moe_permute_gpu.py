@@ -119,6 +119,34 @@ def test_rows_with_a_pitch_and_without_alignment(dtype):
     assert torch.equal(moe.dispatch(one, plan), moe.dispatch(one.contiguous(), plan))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+def test_dispatch_nvfp4_of_rows_with_a_pitch(dtype):
+    from eval_test_b200 import moe
+    plan = moe.plan(choices(37, 5, 2, 0.1, seed=1), 5)
+    wide = _normal((37, 320), dtype, 3)
+    live = plan.slots.reshape(-1)[plan.slots.reshape(-1) >= 0].long()
+    for x in (wide[:, 64:256], wide[3:4, :192].expand(37, 192)):
+        (a, sfa), (b, sfb) = moe.dispatch_nvfp4(x, plan), moe.dispatch_nvfp4(x.contiguous(), plan)
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        s, t = (v.view(torch.uint8).permute(5, 2, 1, 0, 4, 3).reshape(plan.most_tiles * 128, -1)[live] for v in (sfa, sfb))
+        assert torch.equal(s, t)
+
+
+def test_the_same_call_gives_the_same_bits():
+    from eval_test_b200 import moe
+    T, E, k, H = 3000, 40, 6, 1000
+    ids = choices(T, E, k, 0.1, seed=8)
+    y, w, d = _normal((T * k, H), BF16, 1), _normal((T, k), F32, 2), _normal((T, H), BF16, 3)
+
+    def once():
+        plan = moe.plan(ids, E)
+        return (plan.buffer[:3 * (E + 1) + 3 * T * k], moe.combine(y, plan, w), *moe.combine_backward(d, y, plan, w), moe.dispatch_backward(y, plan))
+
+    first = once()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, once()))
+
+
 def test_of_no_tokens_and_no_columns():
     from eval_test_b200 import moe
     plan = moe.plan(torch.empty((0, 2), dtype=torch.int32, device="cuda"), 3)
