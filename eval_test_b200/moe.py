@@ -33,7 +33,7 @@ _KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 class Plan:
     """How the copies of a batch are sorted (``nvfp4_moe_plan``).  One int32 buffer on the batch's device holds its six
     tables; the views are made when they are asked for (a call of the layer needs only their addresses)."""
-    __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "num_copies", "most_tiles", "device", "_at")
+    __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "num_copies", "most_tiles", "_at")
 
     def __init__(self, num_tokens: int, top_k: int, num_experts: int, device: torch.device, more: int = 0):
         n, e = num_tokens * top_k, num_experts + 1
@@ -42,7 +42,7 @@ class Plan:
         size = 3 * e + 3 * n + scratch + more
         # (no copies: nothing is launched, and every expert starts at row 0)
         self.buffer = torch.empty(size, dtype=torch.int32, device=device) if n else torch.zeros(size, dtype=torch.int32, device=device)
-        self.num_tokens, self.top_k, self.num_experts, self.num_copies, self.device = num_tokens, top_k, num_experts, n, device
+        self.num_tokens, self.top_k, self.num_experts, self.num_copies = num_tokens, top_k, num_experts, n
         # 128-row tiles that this many copies can fill at most, whatever their experts
         active = n if n < num_experts else num_experts
         self.most_tiles = active + (n - active) // 128
@@ -115,16 +115,23 @@ def _choices(t: torch.Tensor, name: str, dtype: torch.dtype, shape=None) -> None
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _same_device(device: torch.device, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"all tensors have to be on one device, got {t.device} beside {device}")
+def _same_device(first: torch.Tensor, *others) -> None:
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"all tensors have to be on one device, got {t.device} beside {first.device}")
 
 
-def _call(entry: str, device: torch.device, *args) -> None:
-    """An entry point on the tensors' device and torch's current stream there."""
-    fn, index = getattr(_lib.load(), entry), device.index
-    if torch.cuda.current_device() == index:
+_ENTRIES: dict = {}     # entry points of the library by name
+
+
+def _call(entry: str, like: torch.Tensor, *args) -> None:
+    """An entry point on the device of ``like`` and torch's current stream there."""
+    fn = _ENTRIES.get(entry)
+    if fn is None:
+        fn = _ENTRIES[entry] = getattr(_lib.load(), entry)
+    index = like.get_device()
+    if torch._C._cuda_getDevice() == index:
         code = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
@@ -168,7 +175,7 @@ def plan(experts: torch.Tensor, num_experts: int) -> Plan:
         raise ValueError(f"experts: expected at most {MAX_CHOICES} choices for a token, got {k}")
     p = Plan(T, k, num_experts, experts.device)
     if T * k:
-        _call("nvfp4_moe_plan", experts.device, experts.data_ptr(), T, num_experts, k, *p._at)
+        _call("nvfp4_moe_plan", experts, experts.data_ptr(), T, num_experts, k, *p._at)
     return p
 
 
@@ -189,7 +196,7 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torc
     if mask is not None:
         if mask.dtype != torch.bool or mask.shape != (T,) or not mask.is_contiguous():
             raise ValueError(f"mask: expected a contiguous bool tensor of shape {(T,)}")
-        _same_device(device, mask)
+        _same_device(logits, mask)
     # the weights and the choices lie behind the plan's tables (one allocation: each costs as much as a launch)
     n = T * top_k
     p = Plan(T, top_k, E, device, 2 * n)
@@ -198,7 +205,7 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torc
     experts = p.buffer.as_strided((T, top_k), (top_k, 1), at + n)
     if T:
         address = p._at[0] + 4 * at
-        _call("nvfp4_moe_route", device, logits.data_ptr(), _KINDS[logits.dtype], ld, None if mask is None else mask.data_ptr(),
+        _call("nvfp4_moe_route", logits, logits.data_ptr(), _KINDS[logits.dtype], ld, None if mask is None else mask.data_ptr(),
               T, E, top_k, int(renormalize), address, address + 4 * n, *p._at)
     return Routing(weights, experts, p)
 
@@ -216,10 +223,10 @@ def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, weights: to
     _choices(experts, "experts", torch.int32, (T, k))
     _choices(weights, "weights", torch.float32, (T, k))
     _choices(grad_weights, "grad_weights", torch.float32, (T, k))
-    _same_device(logits.device, weights, experts, grad_weights)
+    _same_device(logits, weights, experts, grad_weights)
     out = logits.new_empty((T, E))
     if T:
-        _call("nvfp4_moe_route_backward", logits.device, grad_weights.data_ptr(), logits.data_ptr(), _KINDS[logits.dtype], ld,
+        _call("nvfp4_moe_route_backward", logits, grad_weights.data_ptr(), logits.data_ptr(), _KINDS[logits.dtype], ld,
               weights.data_ptr(), experts.data_ptr(), T, E, k, int(renormalize), out.data_ptr())
     return out
 
@@ -229,10 +236,10 @@ def dispatch(x: torch.Tensor, plan: Plan) -> torch.Tensor:
     T, k = plan.num_tokens, plan.top_k
     ld = _matrix(x, "x", T)
     H = x.shape[1]
-    _same_device(x.device, plan)
+    _same_device(x, plan.buffer)
     out = x.new_empty((T * k, H))
     if out.numel():
-        _call("nvfp4_moe_dispatch", x.device, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[3], plan._at[0], T,
+        _call("nvfp4_moe_dispatch", x, x.data_ptr(), _KINDS[x.dtype], ld, plan._at[3], plan._at[0], T,
               plan.num_experts, k, H, out.data_ptr())
     return out
 
@@ -253,10 +260,10 @@ def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dt
         raise ValueError(f"dtype: expected float32, float16 or bfloat16, got {dtype}")
     if weights is not None:
         _choices(weights, "weights", torch.float32, (T, k))
-    _same_device(y.device, plan, weights)
+    _same_device(y, plan.buffer, weights)
     out = y.new_empty((T, H), dtype=dtype) if k else y.new_zeros((T, H), dtype=dtype)
     if out.numel() and k:
-        _call("nvfp4_moe_combine", y.device, y.data_ptr(), _KINDS[y.dtype], ld, None if weights is None else weights.data_ptr(),
+        _call("nvfp4_moe_combine", y, y.data_ptr(), _KINDS[y.dtype], ld, None if weights is None else weights.data_ptr(),
               plan._at[3], T, k, H, out.data_ptr(), _KINDS[dtype])
     return out
 
@@ -268,11 +275,11 @@ def combine_backward(grad_out: torch.Tensor, y: torch.Tensor, plan: Plan, weight
     ldo, ld = _matrix(grad_out, "grad_out", T), _matrix(y, "y", T * k, grad_out.shape[1])
     H = y.shape[1]
     _choices(weights, "weights", torch.float32, (T, k))
-    _same_device(y.device, grad_out, plan, weights)
+    _same_device(y, grad_out, plan.buffer, weights)
     dy = y.new_empty((T * k, H))
     dw = torch.empty_like(weights) if H else torch.zeros_like(weights)
     if dy.numel():
-        _call("nvfp4_moe_combine_backward", y.device, grad_out.data_ptr(), _KINDS[grad_out.dtype], ldo, y.data_ptr(), _KINDS[y.dtype],
+        _call("nvfp4_moe_combine_backward", y, grad_out.data_ptr(), _KINDS[grad_out.dtype], ldo, y.data_ptr(), _KINDS[y.dtype],
               ld, weights.data_ptr(), plan._at[3], plan._at[0], T, plan.num_experts, k, H, dy.data_ptr(),
               dw.data_ptr())
     return dy, dw
@@ -287,21 +294,20 @@ def dispatch_nvfp4(x: torch.Tensor, plan: Plan):
     K = x.shape[1]
     if K % 64 or not K:
         raise ValueError(f"x: the width has to be a multiple of 64, got {K}")
-    _same_device(x.device, plan)
+    _same_device(x, plan.buffer)
     packed, scales = _new_operand(x, T * k, plan.most_tiles * 128, K)
     if T * k:
         scratch = _lib.load().nvfp4_moe_dispatch_scratch(T, k, K) if T * k > 1024 else 0
         table = x.new_empty(scratch, dtype=torch.uint8) if scratch else None
         offsets, tiles, _, rows, slots, source, _ = plan._at
-        _call("nvfp4_moe_dispatch_nvfp4", x.device, x.data_ptr(), _KINDS[x.dtype], ld, offsets, tiles, rows, slots, source, T,
+        _call("nvfp4_moe_dispatch_nvfp4", x, x.data_ptr(), _KINDS[x.dtype], ld, offsets, tiles, rows, slots, source, T,
               plan.num_experts, k, K, packed.data_ptr(), scales.data_ptr(), table.data_ptr() if scratch else None)
     return packed, scales
 
 
 def _products(a, sfa, weights, plan: Plan, alpha):
-    """Checks the operands of an expert product -> (pointers in the C order, alphas pointer, alpha, R, E, N, K, device)."""
+    """Checks the operands of an expert product -> (pointers in the C order, alphas pointer, alpha, R, E, N, K)."""
     R, E = plan.num_copies, plan.num_experts
-    device = a.device
     if a.dim() != 3 or not a.is_cuda:
         raise ValueError("a: expected the CUDA operand [T * k, K/2, 1] that dispatch_nvfp4 returns")
     K, N = 2 * a.shape[1], weights[0].shape[0]
@@ -312,42 +318,42 @@ def _products(a, sfa, weights, plan: Plan, alpha):
     ptrs = [_operand(a, R, K // 2, 1, "a"), _scales(sfa, plan.most_tiles * 128, K, 1, "sfa")]
     for i in range(0, len(weights), 2):
         ptrs += [_operand(weights[i], N, K // 2, E, "b"), _scales(weights[i + 1], N, K, E, "sfb")]
-    _same_device(device, sfa, *weights, plan)
+    _same_device(a, sfa, *weights, plan.buffer)
     alphas = None
     if isinstance(alpha, torch.Tensor):
         if alpha.dtype != torch.float32 or alpha.shape != (E,) or not alpha.is_contiguous():
             raise ValueError(f"alpha: expected a number or a contiguous float32 tensor of shape {(E,)}")
-        _same_device(device, alpha)
+        _same_device(a, alpha)
         alphas, alpha = alpha.data_ptr(), 1.0
-    return ptrs + [*plan._at[:3], alphas], float(alpha), R, E, N, K, device
+    return ptrs + [*plan._at[:3], alphas], float(alpha), R, E, N, K
 
 
 def expert_gemm(a, sfa, b, sfb, plan: Plan, alpha=1.0) -> torch.Tensor:
     """``y[r] = fp16(alpha_e * a[r] @ b_e^T)`` for every sorted row r of expert e -> fp16 [T * k, N].  ``a``, ``sfa`` as
     ``dispatch_nvfp4`` or ``expert_dual_gemm_nvfp4`` returns them, ``b`` [N, K/2, E] with its 6-D scales; ``alpha`` a number
     or a float32 tensor [E], the experts' global scales.  N is a multiple of 128, K of 256."""
-    ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b, sfb), plan, alpha)
+    ptrs, alpha, R, E, N, K = _products(a, sfa, (b, sfb), plan, alpha)
     c = a.new_empty((R, N), dtype=torch.float16)
     if R:
-        _call("nvfp4_moe_gemm", device, *ptrs, c.data_ptr(), R, E, N, K, alpha)
+        _call("nvfp4_moe_gemm", a, *ptrs, c.data_ptr(), R, E, N, K, alpha)
     return c
 
 
 def expert_dual_gemm(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0) -> torch.Tensor:
     """``fp16(silu(alpha_e * a[r] @ b1_e^T) * (alpha_e * a[r] @ b2_e^T))`` -> fp16 [T * k, N]; arguments as for
     ``expert_gemm``."""
-    ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
+    ptrs, alpha, R, E, N, K = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
     c = a.new_empty((R, N), dtype=torch.float16)
     if R:
-        _call("nvfp4_moe_dual_gemm", device, *ptrs, c.data_ptr(), R, E, N, K, alpha)
+        _call("nvfp4_moe_dual_gemm", a, *ptrs, c.data_ptr(), R, E, N, K, alpha)
     return c
 
 
 def expert_dual_gemm_nvfp4(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0):
     """``expert_dual_gemm`` with its rows quantised to NVFP4, bit for bit what quantising the fp16 rows gives -> (operand
     ``[T * k, N/2, 1]``, 6-D scales): ``a`` and ``sfa`` of the next product of the same plan."""
-    ptrs, alpha, R, E, N, K, device = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
+    ptrs, alpha, R, E, N, K = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
     packed, scales = _new_operand(a, R, plan.most_tiles * 128, N)
     if R:
-        _call("nvfp4_moe_dual_gemm_nvfp4", device, *ptrs, packed.data_ptr(), scales.data_ptr(), R, E, N, K, alpha)
+        _call("nvfp4_moe_dual_gemm_nvfp4", a, *ptrs, packed.data_ptr(), scales.data_ptr(), R, E, N, K, alpha)
     return packed, scales
