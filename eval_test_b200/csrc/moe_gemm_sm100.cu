@@ -21,8 +21,8 @@
 //     tokens only, and the instruction with 128 columns reads its weights from shared memory twice as often as it can:
 //     547 us for 512 rows per expert, N = 2048, K = 7168, against 440 us.)  silu(x) waits in registers for y;
 //   * persistent pairs; column tile fastest, so that the pairs that run together share an expert's tokens in L2;
-//   * warp 0 = TMA producer (both CTAs, own rows; every load counts its bytes on the leader's barrier), warp 1 = MMA
-//     issuer (leader), the others = epilogue, NT / 64 warps per TMEM lane quadrant with two chunks of 32 tokens each (eight
+//   * warps 0 and 2 = TMA producers of the weights and of the tokens (both CTAs, own rows; every load counts its bytes on
+//     the leader's barrier), warp 1 = MMA issuer (leader), warps 4.. = epilogue, NT / 64 warps per TMEM lane quadrant with two chunks of 32 tokens each (eight
 //     warps with 128 values of silu(x) each left their exponentials no room to overlap: 15 000 cycles per tile, as long as
 //     the products of K = 4096); a stage is 256 K elements: 16 KB of weights, 128 bytes per token (in boxes of 128, 64, 32
 //     and 16 rows), scale atoms;
@@ -56,7 +56,8 @@ constexpr int XM = 128;                              // weight rows of a CTA and
 constexpr int X_PITCH = 144;                         // bytes of two tokens' 32 outputs in a turning buffer (128 + bank spread)
 constexpr uint32_t X_TURN_BYTES = 8 * X_PITCH;       // of one epilogue warp
 __host__ __device__ constexpr int x_epilogue_warps(int nt) { return 4 * (nt / 64); }
-__host__ __device__ constexpr int x_threads(int nt) { return 64 + 32 * x_epilogue_warps(nt); }
+constexpr int X_FIRST_EPILOGUE = 4;                 // warps before it: weights producer, MMA issuer, tokens producer, idle
+__host__ __device__ constexpr int x_threads(int nt) { return 32 * (X_FIRST_EPILOGUE + x_epilogue_warps(nt)); }
 
 template <int NT>
 struct ExpertStage {                                 // one stage of one CTA
@@ -117,6 +118,11 @@ struct ExpertTables {
         return ti;
     }
 };
+
+// A shared-memory descriptor `units` of 16 bytes behind another one (no carry out of the low word: see the assertion).
+__device__ __forceinline__ uint64_t desc_at(uint64_t first, uint32_t units) {
+    return (first & 0xffffffff00000000ull) | ((uint32_t)first + units);
+}
 
 // What one epilogue warp does with the accumulator of one pass: its 32 weight rows (lanes) of the two 32-token chunks
 // group and group + NT / 64.  Columns of the chunks [lo, hi) are shared with the other accumulator: they are read first
@@ -216,7 +222,7 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
-            mbar_init(full0 + 8 * s, 1);                        // the leader's copy: one arrival + both CTAs' bytes
+            mbar_init(full0 + 8 * s, 2);                        // the leader's copy: its producers + both CTAs' bytes
             mbar_init(empty0 + 8 * s, 1);
         }
         for (int b = 0; b < 2; b++) {
@@ -256,10 +262,12 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     const int kiters = p.K / BK, apb = p.K / 64;                // K steps; scale atoms of a 128-row block
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
 
-    if (warp == 0) {
-        // ------------------------------------------------------------------ producer (both CTAs, own rows)
+    if (warp == 0 || warp == 2) {
+        // ------------------------------------------------------------------ producers (both CTAs, own rows): warp 0 the
+        // weights, warp 2 the tokens (issuing a copy takes a thread about 70 cycles, and a stage has up to ten)
         if (elect_one()) {
-            uint32_t it = 0;
+            const bool weights = warp == 0;
+            uint32_t slot = 0, phase = 1;
             bool alive = true;
             const uint32_t leader_full0 = mapa_shared(full0, 0);
             for (int t = pair; alive && t < total_tiles; t += npairs) {
@@ -271,41 +279,52 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
                 const int atom_w = (ti.e * (p.N / XM) + ti.w) * apb, atom_t = ti.atoms * apb;
                 // the leader announces the bytes of both CTAs.  Weight rows beyond N (second CTA of the last column) read
                 // as zeros; their scale block does not exist and is not fetched
-                const uint32_t tx = 2u * (Stage::W + (uint32_t)half * 128u + (uint32_t)atoms * 2048u) + (peer_exists ? 2u : 1u) * Stage::SFW;
-                for (int step = 0; step < PASSES * kiters; step++, it++) {
-                    const int slot = it % STAGES;
-                    if (!mbar_wait_cluster(empty0 + 8 * slot, ((it / STAGES) & 1) ^ 1, p.budget_ns)) {
-                        report_status(p.status, DEV_TIMEOUT_PRODUCER);
-                        alive = false;
-                        break;
-                    }
-                    const bool second = DUAL && step >= kiters;
-                    const uint32_t full = leader_full0 + 8 * slot;
-                    const uint32_t sW = smem0 + slot * Stage::BYTES, sT = sW + Stage::W;
-                    const uint32_t sSFW = sT + Stage::T, sSFT = sSFW + Stage::SFW;
-                    const int k0 = (step - (second ? kiters : 0)) * BK, ka = k0 / 64;
-                    if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * slot, tx);
-                    tma_load_3d_pair(sW, second ? &maps.b2 : &maps.b, k0, ti.w * XM, ti.e, full);
-                    int r = 0;
-#pragma unroll
-                    for (int b = 0; b < 4; b++)
-                        if (half & (128 >> b)) {
-                            tma_load_3d_pair(sT + r * 128, &maps.a[b], k0, row0 + r, 0, full);
-                            r += 128 >> b;
+                const uint32_t tx = weights ? 2u * Stage::W + (peer_exists ? 2u : 1u) * Stage::SFW
+                                            : 2u * ((uint32_t)half * 128u + (uint32_t)atoms * 2048u);
+                for (int pass = 0; alive && pass < PASSES; pass++) {
+                    const CUtensorMap *map_w = pass ? &maps.b2 : &maps.b, *map_sw = pass ? &maps.sb2 : &maps.sb;
+                    for (int kit = 0; kit < kiters; kit++) {
+                        if (!mbar_wait_cluster(empty0 + 8 * slot, phase, p.budget_ns)) {
+                            report_status(p.status, DEV_TIMEOUT_PRODUCER);
+                            alive = false;
+                            break;
                         }
-                    if (block_exists) tma_load_2d_pair(sSFW, second ? &maps.sb2 : &maps.sb, 0, atom_w + ka, full);
-                    for (int j = 0; j < atoms; j++) tma_load_2d_pair(sSFT + j * 2048u, &maps.sa, 0, atom_t + j * apb + ka, full);
+                        const uint32_t full = leader_full0 + 8 * slot;
+                        const uint32_t sW = smem0 + slot * Stage::BYTES, sT = sW + Stage::W;
+                        const uint32_t sSFW = sT + Stage::T, sSFT = sSFW + Stage::SFW;
+                        const int k0 = kit * BK, ka = kit * (BK / 64);
+                        if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * slot, tx);
+                        if (weights) {
+                            tma_load_3d_pair(sW, map_w, k0, ti.w * XM, ti.e, full);
+                            if (block_exists) tma_load_2d_pair(sSFW, map_sw, 0, atom_w + ka, full);
+                        } else {
+                            int r = 0;
+#pragma unroll
+                            for (int b = 0; b < 4; b++)
+                                if (half & (128 >> b)) {
+                                    tma_load_3d_pair(sT + r * 128, &maps.a[b], k0, row0 + r, 0, full);
+                                    r += 128 >> b;
+                                }
+                            for (int j = 0; j < atoms; j++) tma_load_2d_pair(sSFT + j * 2048u, &maps.sa, 0, atom_t + j * apb + ka, full);
+                        }
+                        if (++slot == STAGES) { slot = 0; phase ^= 1; }
+                    }
                 }
             }
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------------ leader: MMA issuer for the pair (one lane)
         if (elect_one() && rank == 0) {
-            uint32_t it = 0, seq = 0;                           // stages and passes so far
+            // One thread issues everything, so what it computes per instruction counts: the descriptors of a stage differ
+            // from those of the first one by their address field, the low bits of the low word.
+            const uint64_t d_w0 = make_desc_k_sw128(smem0), d_t0 = make_desc_k_sw128(smem0 + Stage::W);
+            const uint64_t d_sfw0 = make_desc_sf(smem0 + Stage::W + Stage::T), d_sft0 = make_desc_sf(smem0 + Stage::W + Stage::T + Stage::SFW);
+            static_assert(STAGES * Stage::BYTES < (1u << 18), "the address field holds 18 bits");
+            uint32_t slot = 0, phase = 0, odd = 0, seq = 0;     // ring slot and its phase, scale region, passes so far
             bool alive = true;
             for (int t = pair; alive && t < total_tiles; t += npairs) {
                 const ExpertTile ti = where.locate<NT>(t, rank);
-                const int atoms = (ti.n + 127) / 128;
+                const bool two_atoms = ti.n > 128;
                 const uint32_t idesc = make_idesc_nvfp4(2 * XM, (ti.n + 31) & ~31);
                 for (int pass = 0; alive && pass < PASSES; pass++, seq++) {
                     const uint32_t buf = seq & 1;
@@ -318,38 +337,40 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
                     }
                     tc_fence_after_sync();
                     const uint32_t t_acc = tmem_base + buf * ACC1_OFF;
-                    for (int kit = 0; kit < kiters; kit++, it++) {
-                        const int slot = it % STAGES;
-                        if (!mbar_wait_cluster(full0 + 8 * slot, (it / STAGES) & 1, p.budget_ns)) {   // both CTAs' bytes
+                    for (int kit = 0; kit < kiters; kit++) {
+                        if (!mbar_wait_cluster(full0 + 8 * slot, phase, p.budget_ns)) {   // both CTAs' bytes
                             report_status(p.status, DEV_TIMEOUT_CONSUMER);
                             alive = false;
                             break;
                         }
                         tc_fence_after_sync();
-                        const uint32_t sW = smem0 + slot * Stage::BYTES, sT = sW + Stage::W;
-                        const uint32_t sSFW = sT + Stage::T, sSFT = sSFW + Stage::SFW;
-                        const uint32_t t_sfw = tmem_base + SF_BASE + (it & 1) * SF_COLS, t_sft = t_sfw + 16;
+                        const uint32_t at = slot * (Stage::BYTES >> 4);
+                        const uint32_t t_sfw = tmem_base + SF_BASE + odd * SF_COLS, t_sft = t_sfw + 16;
 #pragma unroll
                         for (int ks = 0; ks < 4; ks++) {
-                            tc_cp_sf_atom_pair(t_sfw + 4 * ks, make_desc_sf(sSFW + 512 * ks));
+                            tc_cp_sf_atom_pair(t_sfw + 4 * ks, desc_at(d_sfw0, at + 32 * ks));
+                            tc_cp_sf_atom_pair(t_sft + ks * (NT / 32), desc_at(d_sft0, at + 32 * ks));
+                        }
+                        if (NT > 128 && two_atoms) {
 #pragma unroll
-                            for (int j = 0; j < NT / 128; j++)
-                                if (j < atoms) tc_cp_sf_atom_pair(t_sft + ks * (NT / 32) + 4 * j, make_desc_sf(sSFT + 2048 * j + 512 * ks));
+                            for (int ks = 0; ks < 4; ks++) tc_cp_sf_atom_pair(t_sft + ks * (NT / 32) + 4, desc_at(d_sft0, at + 128 + 32 * ks));
                         }
 #pragma unroll
                         for (int ks = 0; ks < 4; ks++)
-                            tc_mma_nvfp4_pair(t_acc, make_desc_k_sw128(sW + 32 * ks), make_desc_k_sw128(sT + 32 * ks), idesc,
-                                              t_sfw + 4 * ks, t_sft + ks * (NT / 32), (kit | ks) != 0 ? 1u : 0u);
+                            tc_mma_nvfp4_pair(t_acc, desc_at(d_w0, at + 2 * ks), desc_at(d_t0, at + 2 * ks), idesc, t_sfw + 4 * ks,
+                                              t_sft + ks * (NT / 32), (kit | ks) != 0 ? 1u : 0u);
                         tc_commit_pair(empty0 + 8 * slot, 3);               // frees the stage in both CTAs
+                        odd ^= 1;
+                        if (++slot == STAGES) { slot = 0; phase ^= 1; }
                     }
                     if (alive) tc_commit_pair(acc_full0 + 8 * buf, 3);      // accumulators complete in both CTAs
                 }
             }
         }
-    } else {
+    } else if (warp >= X_FIRST_EPILOGUE) {
         // ------------------------------------------------------------------ epilogue warps (both CTAs)
-        const int q = warp & 3, group = (warp - 2) >> 2; // TMEM lane quadrant this warp may access; which chunks it takes
-        uint8_t* turn = smem_raw + (smem0 - smem_u32(smem_raw)) + STAGES * Stage::BYTES + (warp - 2) * X_TURN_BYTES;
+        const int q = warp & 3, group = (warp - X_FIRST_EPILOGUE) >> 2; // TMEM lane quadrant this warp may access; which chunks it takes
+        uint8_t* turn = smem_raw + (smem0 - smem_u32(smem_raw)) + STAGES * Stage::BYTES + (warp - X_FIRST_EPILOGUE) * X_TURN_BYTES;
         const uint32_t l_acc_empty0 = mapa_shared(acc_empty0, 0), l_ovl_free = mapa_shared(ovl_free, 0);
         {
             // rows behind the last copy (choices that were dropped): zero, so that sums over the buffer are sums over copies
@@ -357,7 +378,7 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             const uint32_t zero[8] = {};
             const size_t end = (size_t)p.R * row_bytes / 32;
             constexpr int THREADS = 32 * x_epilogue_warps(NT);
-            for (size_t i = (size_t)live_rows * row_bytes / 32 + (size_t)blockIdx.x * THREADS + threadIdx.x - 64; i < end;
+            for (size_t i = (size_t)live_rows * row_bytes / 32 + (size_t)blockIdx.x * THREADS + threadIdx.x - 32 * X_FIRST_EPILOGUE; i < end;
                  i += (size_t)gridDim.x * THREADS)
                 st_global_256(p.c + i * 32, zero);
         }
