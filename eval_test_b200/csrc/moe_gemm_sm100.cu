@@ -32,8 +32,8 @@
 //     to fp16, are turned over in a piece of shared memory that belongs to the warp, 16 tokens x 32 weight rows at a time,
 //     and a lane stores 16 of a token's outputs (32 bytes), or quantises them (they are one block).
 // Every mbarrier wait is bounded; on expiry the role records a status code and leaves its loop, the CTA still frees its
-// tensor memory and exits.  The two hardware cluster barriers (after set-up, before exit) are reached by every thread on
-// every path.
+// tensor memory and exits.  The epilogue's named barrier is reached by all of its warps or by none; the two hardware cluster
+// barriers (after set-up, before exit) are reached by every thread on every path.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -211,6 +211,7 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     // same layout in both CTAs (remote arrivals and pair-wide commits address barriers by offset)
     __shared__ __align__(8) uint64_t bars[2 * STAGES + 5];
     __shared__ uint32_t tmem_base_slot;
+    __shared__ int gave_up;
 
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -230,6 +231,7 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             mbar_init(acc_empty0 + 8 * b, 2 * x_epilogue_warps(NT));
         }
         mbar_init(ovl_free, 2 * x_epilogue_warps(NT));
+        gave_up = 0;
         fence_mbar_init();
         prefetch_tmap(&maps.a[0]);
         prefetch_tmap(&maps.a[3]);
@@ -395,8 +397,17 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             for (int pass = 0; pass < PASSES; pass++, seq++) {
                 const uint32_t buf = seq & 1;
                 if (!alive) break;
-                if (!mbar_wait(acc_full0 + 8 * buf, (seq >> 1) & 1, p.budget_ns)) {
-                    if (lane == 0) report_status(p.status, DEV_TIMEOUT_EPILOGUE);
+                // one warp waits for the accumulator and the others for that warp (sixteen waiting warps took power from the
+                // rest of the board: 1 %).  If it gives up it says in which pass, so that all of them leave at the same barrier
+                if (warp == X_FIRST_EPILOGUE && !mbar_wait(acc_full0 + 8 * buf, (seq >> 1) & 1, p.budget_ns)) {
+                    if (lane == 0) {
+                        report_status(p.status, DEV_TIMEOUT_EPILOGUE);
+                        *(volatile int*)&gave_up = (int)seq + 1;
+                    }
+                    __syncwarp();
+                }
+                named_bar_sync(1, 32 * x_epilogue_warps(NT));
+                if (*(volatile int*)&gave_up == (int)seq + 1) {
                     alive = false;
                     break;
                 }
