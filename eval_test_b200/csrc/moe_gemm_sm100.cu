@@ -6,8 +6,8 @@
 // The roles are exchanged against the GEMM kernels: the WEIGHTS are the 128-row operand of the tensor core instruction
 // and the tokens its N side, whose width is any multiple of 16.  An expert has any number of tokens, so with the tokens
 // as 128-row tiles a layer of about 128 tokens per expert computes half as much again on rows that do not exist, at a
-// clock that the board's power limit sets (64 experts, 8192 copies, N = 4096, K = 7168: 220 us that way, 204 us
-// this way; 1.14 GB at the measured copy rate take 175 us).  An expert's rows start anywhere in A: a TMA box may start
+// clock that the board's power limit sets (64 experts, 8192 copies, N = 4096, K = 7168: 215 us that way, 195 us
+// this way on a cool board, 253 and 225 us after a second of it; 1.14 GB at the measured copy rate take 175 us).  An expert's rows start anywhere in A: a TMA box may start
 // at any row, and what it reads of the next expert's rows is multiplied but not stored.
 //
 //   * CTA PAIRS (cluster of 2, cta_group::2, as in gemm_pair_kernel): a tile is 256 weight rows x NT tokens of one
@@ -19,13 +19,13 @@
 //     flight) where they have few;
 //   * DUAL: two passes over K, x into one accumulator and y into the other.  (Both products in one pass leave TMEM for 128
 //     tokens only, and the instruction with 128 columns reads its weights from shared memory twice as often as it can:
-//     547 us for 512 rows per expert, N = 2048, K = 7168, against 440 us.)  silu(x) waits in registers for y;
+//     547 us for 512 rows per expert, N = 2048, K = 7168, against 406 us.)  silu(x) waits in registers for y;
 //   * persistent pairs; column tile fastest, so that the pairs that run together share an expert's tokens in L2;
 //   * warps 0 and 2 = TMA producers of the weights and of the tokens (both CTAs, own rows; every load counts its bytes on
-//     the leader's barrier), warp 1 = MMA issuer (leader), warps 4.. = epilogue, NT / 64 warps per TMEM lane quadrant with two chunks of 32 tokens each (eight
-//     warps with 128 values of silu(x) each left their exponentials no room to overlap: 15 000 cycles per tile, as long as
-//     the products of K = 4096); a stage is 256 K elements: 16 KB of weights, 128 bytes per token (in boxes of 128, 64, 32
-//     and 16 rows), scale atoms;
+//     the leader's barrier), warp 1 = MMA issuer (leader), warps 4.. = epilogue, NT / 64 warps per TMEM lane quadrant with
+//     two chunks of 32 tokens each (eight warps with 128 values of silu(x) each left their exponentials no room to overlap:
+//     15 000 cycles per tile, as long as the products of K = 4096); a stage is 256 K elements: 16 KB of weights, 128 bytes
+//     per token (in boxes of 128, 64, 32 and 16 rows), scale atoms;
 //   * accumulators in TMEM, lane = weight row, column = token; two of them, which with 256 columns each share 96 that the
 //     epilogue drains first (512 columns do not hold both and the scales);
 //   * epilogue: the accumulator goes to registers at once, which frees it for the next pass but one; the results, rounded

@@ -51,6 +51,9 @@ class Plan:
         # addresses: offsets, tiles, wide_tiles, rows, slots, source, scratch
         self._at = (base, base + 4 * e, base + 8 * e, rows, rows + 4 * n, rows + 8 * n, rows + 12 * n)
 
+    def __reduce__(self):
+        raise TypeError("a Plan holds addresses of its buffer: it cannot be copied or pickled, make it again from the choices")
+
     def _per_expert(self, i: int) -> torch.Tensor:
         e = self.num_experts + 1
         return self.buffer.as_strided((e,), (1,), i * e)
@@ -297,7 +300,7 @@ def dispatch_nvfp4(x: torch.Tensor, plan: Plan):
     _same_device(x, plan.buffer)
     packed, scales = _new_operand(x, T * k, plan.most_tiles * 128, K)
     if T * k:
-        scratch = _lib.load().nvfp4_moe_dispatch_scratch(T, k, K) if T * k > 1024 else 0
+        scratch = _lib.load().nvfp4_moe_dispatch_scratch(T, k, K) if T * k * K >= 1 << 24 else 0
         table = x.new_empty(scratch, dtype=torch.uint8) if scratch else None
         offsets, tiles, _, rows, slots, source, _ = plan._at
         _call("nvfp4_moe_dispatch_nvfp4", x, x.data_ptr(), _KINDS[x.dtype], ld, offsets, tiles, rows, slots, source, T,

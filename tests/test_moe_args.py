@@ -74,3 +74,13 @@ def test_most_tiles_bounds_every_distribution():
         p = moe.Plan(copies, 1, E, torch.device("cpu"))
         reached = max(tiles((*c, copies - sum(c))) for c in product(range(copies + 1), repeat=E - 1) if sum(c) <= copies)
         assert p.most_tiles == reached, (copies, E)
+
+
+def test_a_plan_is_not_copied():
+    import copy
+    import pickle
+    from eval_test_b200 import moe
+    p = moe.Plan(4, 2, 8, torch.device("cpu"))
+    for f in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="Plan"):
+            f(p)

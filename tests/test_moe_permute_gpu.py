@@ -162,7 +162,8 @@ def test_of_no_tokens_and_no_columns():
 
 
 @pytest.mark.parametrize("T,E,k,K", [(1, 1, 1, 64), (1, 64, 8, 4096), (40, 7, 3, 192), (300, 2, 2, 256), (33, 300, 4, 1024),
-                                     (1030, 1000, 8, 2304), (9000, 3, 2, 1024), (17000, 9, 8, 320), (10300, 37, 8, 2048)])
+                                     (1030, 1000, 8, 2304), (9000, 3, 2, 1024), (17000, 9, 8, 320), (10300, 37, 8, 2048),
+                                     (128, 40, 8, 163840)])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("drop", [0.0, 0.4])
 def test_dispatch_nvfp4_is_the_quantiser_of_the_sorted_rows(T, E, k, K, dtype, drop):
