@@ -295,6 +295,35 @@ def test_layer_on_two_streams_at_once():
     _ok_status()
 
 
+def test_an_event_between_two_calls_is_waited_for():
+    """The kernels may start before the one in front of them has ended, but not before an event of another stream."""
+    from eval_test_b200 import moe
+    T, E, k, H = 500, 8, 2, 512
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.zeros((T, H), device="cuda")
+    new = torch.randn((T, H), generator=g, device="cuda")
+    ids = choices(T, E, k, seed=1)
+    plan = moe.plan(ids, E)
+    want = moe.dispatch(new, plan)
+    moe.dispatch_nvfp4(x, plan)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(3):
+        x.zero_()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(a):
+            torch.cuda._sleep(2_000_000)                            # a millisecond, then the copy
+            x.copy_(new)
+            ready = a.record_event()
+        with torch.cuda.stream(b):
+            plan = moe.plan(ids, E)
+            b.wait_event(ready)
+            xs = moe.dispatch(x, plan)
+            back = moe.combine(xs, plan)
+        torch.cuda.synchronize()
+        assert torch.equal(xs, want) and torch.equal(back, new + new)
+
+
 def test_refusals():
     from eval_test_b200 import moe
     plan, a, sfa, (b, sfb), _, _ = _operands(6, 4, 2, 256, 512, 0.0)
