@@ -17,6 +17,9 @@ namespace nvfp4 {
 
 constexpr int MOE_MAX_EXPERTS = 1024;
 constexpr int MOE_MAX_CHOICES = 32;
+// Copies, and elements of a row: a loop's stride (at most 148 x 8 x 8 warps of four tokens) or 128 rows for each of 1024
+// experts may be added to an index without leaving 31 bits.
+constexpr long long MOE_MOST = (1ll << 31) - (1ll << 20);
 
 // KIND: the element type codes of the C ABI (NVFP4_F32 / NVFP4_F16 / NVFP4_BF16).
 template <int KIND> struct ElemOf { using type = float; };

@@ -340,7 +340,7 @@ int current_device(int* dev) {
 
 int check_sizes(int T, int k, int H, long long ld) {
     if (T <= 0 || k <= 0 || H <= 0 || ld < 0) return NVFP4_ERR_SHAPE;
-    if (k > MOE_MAX_CHOICES || (long long)T * k >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
+    if (k > MOE_MAX_CHOICES || (long long)T * k > MOE_MOST || H > MOE_MOST) return NVFP4_ERR_UNSUPPORTED;
     return NVFP4_OK;
 }
 

@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(PLAN_WARPS * 32, 1) plan_kernel(const PlanArgs
     int fewest = (31 + p.k) / p.k;
     if constexpr (!std::is_void_v<L>) fewest = max(fewest, L::PER_WARP);
     const TokenRange own_tokens = warp_tokens(block_tokens(p.T, ctas, rank), fewest, warp);
-    const int begin = own_tokens.begin * p.k, end = own_tokens.end * p.k;    // (T * k < 2^31: checked by the caller)
+    const int begin = own_tokens.begin * p.k, end = own_tokens.end * p.k;    // (T * k <= MOE_MOST: checked by the caller)
 
     for (int i = threadIdx.x; i < (PLAN_WARPS + 2) * p.E; i += blockDim.x) hist[i] = 0;
     pdl_wait();
@@ -554,7 +554,7 @@ int rows_wide(const void* logits, int kind, long long ld) { return ((uintptr_t)l
 int check_route(int kind, long long ld, int T, int E, int k) {
     if (!kind_ok(kind)) return NVFP4_ERR_UNSUPPORTED;
     if (T <= 0 || E <= 0 || k <= 0 || k > E || ld < 0) return NVFP4_ERR_SHAPE;
-    if (E > MOE_MAX_EXPERTS || k > MOE_MAX_CHOICES || (long long)T * k >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
+    if (E > MOE_MAX_EXPERTS || k > MOE_MAX_CHOICES || (long long)T * k > MOE_MOST) return NVFP4_ERR_UNSUPPORTED;
     return NVFP4_OK;
 }
 
@@ -571,9 +571,7 @@ extern "C" int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* of
                               void* slots, void* source, void* scratch, void* stream) {
     if (!experts || !offsets || !tiles || !wide_tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
     if (T <= 0 || E <= 0 || k <= 0) return NVFP4_ERR_SHAPE;
-    if (k > MOE_MAX_CHOICES) return NVFP4_ERR_UNSUPPORTED;
-    // (padded rows are counted in 32 bits: up to 127 more for every expert)
-    if (E > MOE_MAX_EXPERTS || (long long)T * k + 128ll * E >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
+    if (E > MOE_MAX_EXPERTS || k > MOE_MAX_CHOICES || (long long)T * k > MOE_MOST) return NVFP4_ERR_UNSUPPORTED;
     if (nvfp4_moe_plan_scratch(T, E, k) && !scratch) return NVFP4_ERR_NULL;
     const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)wide_tiles, (int*)rows, (int*)slots, (int*)source, (uint32_t*)scratch, T, E, k};
     return plan_choices(p, (cudaStream_t)stream);
@@ -585,7 +583,6 @@ extern "C" int nvfp4_moe_route(const void* logits, int kind, long long ld, const
     if (!logits || !weights || !experts || !offsets || !tiles || !wide_tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
     int rc = check_route(kind, ld, T, E, k);
     if (rc) return rc;
-    if ((long long)T * k + 128ll * E >= (1ll << 31)) return NVFP4_ERR_UNSUPPORTED;
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;

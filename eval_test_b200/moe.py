@@ -27,6 +27,7 @@ import torch
 from . import _args, _lib, formats as F
 
 MAX_EXPERTS, MAX_CHOICES = 1024, 32
+MAX_COPIES = (1 << 31) - (1 << 20)      # also of a matrix: rows, columns
 _KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
@@ -37,6 +38,8 @@ class Plan:
 
     def __init__(self, num_tokens: int, top_k: int, num_experts: int, device: torch.device, more: int = 0):
         n, e = num_tokens * top_k, num_experts + 1
+        if n > MAX_COPIES:
+            raise ValueError(f"expected at most {MAX_COPIES} choices in a batch, got {n}")
         # behind the tables: the copies per expert of each block of a large sort, then `more` words for the caller
         scratch = _lib.load().nvfp4_moe_plan_scratch(num_tokens, num_experts, top_k) // 4 if n > 4096 else 0
         size = 3 * e + 3 * n + scratch + more
@@ -103,6 +106,8 @@ def _matrix(t: torch.Tensor, name: str, rows: int | None = None, cols: int | Non
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _KINDS):
         raise ValueError(f"{name}: expected a CUDA float32 / float16 / bfloat16 matrix")
     have_rows, have_cols = t.shape
+    if have_rows > MAX_COPIES or have_cols > MAX_COPIES:
+        raise ValueError(f"{name}: expected at most {MAX_COPIES} rows and columns, got {tuple(t.shape)}")
     if (rows is not None and have_rows != rows) or (cols is not None and have_cols != cols):
         raise ValueError(f"{name}: expected shape {(rows, cols)}, got {tuple(t.shape)}")
     pitch, step = t.stride()

@@ -44,6 +44,24 @@ def test_c_entries_reject_bad_arguments(lib):
     assert lib.nvfp4_moe_dual_gemm_nvfp4(P, P, P, P, P, P, P, P, P, None, P, None, 8, 4, 128, 256, 1.0, None) == -1
 
 
+def test_sizes_that_an_index_and_a_loop_s_stride_could_carry_past_31_bits_are_refused(lib):
+    from eval_test_b200 import moe
+    P, plan, most = 32, (32,) * 7, (1 << 31) - (1 << 20)
+    assert moe.MAX_COPIES == most
+    for T, E, k in ((most + 1, 1, 1), ((1 << 31) - 129, 1, 1), (most // 2 + 1, 8, 2)):
+        assert lib.nvfp4_moe_plan(P, T, E, k, *plan, None) == -6
+        assert lib.nvfp4_moe_route(P, 2, 8, None, T, E, k, 1, P, P, *plan, None) == -6
+        assert lib.nvfp4_moe_route_backward(P, P, 2, 8, P, P, T, E, k, 1, P, None) == -6
+        assert lib.nvfp4_moe_dispatch(P, 2, 8, P, P, T, E, k, 8, P, None) == -6
+        assert lib.nvfp4_moe_combine(P, 2, 8, None, P, T, k, 8, P, 2, None) == -6
+    H = most + 1
+    assert lib.nvfp4_moe_dispatch(P, 2, H, P, P, 1, 8, 1, H, P, None) == -6
+    assert lib.nvfp4_moe_combine(P, 2, H, None, P, 1, 1, H, P, 2, None) == -6
+    assert lib.nvfp4_moe_combine_backward(P, 2, H, P, 2, H, P, P, P, 1, 8, 1, H, P, P, None) == -6
+    with pytest.raises(ValueError, match="choices"):          # (past 32 bits the entry would see the low word)
+        moe.Plan(1 << 32, 1, 8, torch.device("cpu"))
+
+
 def test_python_entries_take_cuda_tensors_of_the_documented_types():
     from eval_test_b200 import moe
     x = torch.zeros((4, 64))

@@ -67,10 +67,13 @@ def test_route_ties_infinities_nan_and_empty_rows(T, renormalize):
 
 
 def test_route_rows_with_a_pitch_and_without_alignment():
+    from eval_test_b200 import moe
     big = _logits(50, 201, BF16, 3)
     _check(big[:, 1:100], 4, True)
     _check(big[::3, 7:8], 1, False)
     _check(big[5:6, :].expand(9, 201), 3, True)                     # one row for all tokens
+    with pytest.raises(ValueError, match="at most"):                # (and for more than 32 bits count)
+        moe.route(big[5:6, :].expand((1 << 32) + 5, 201), 3)
 
 
 def test_route_of_no_tokens():
