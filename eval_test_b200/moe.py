@@ -205,12 +205,13 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torc
         if mask.dtype != torch.bool or mask.shape != (T,) or not mask.is_contiguous():
             raise ValueError(f"mask: expected a contiguous bool tensor of shape {(T,)}")
         _same_device(logits, mask)
-    # the weights and the choices lie behind the plan's tables (one allocation: each costs as much as a launch)
+    # the weights and the choices lie behind the plan's tables (one allocation: each costs as much as a launch).  `.data`:
+    # tensors of their own for autograd, so that weights changed in place do not pass for changed choices or tables
     n = T * top_k
     p = Plan(T, top_k, E, device, 2 * n)
     at = p.buffer.shape[0] - 2 * n
-    weights = p.buffer.view(torch.float32).as_strided((T, top_k), (top_k, 1), at)
-    experts = p.buffer.as_strided((T, top_k), (top_k, 1), at + n)
+    weights = p.buffer.view(torch.float32).as_strided((T, top_k), (top_k, 1), at).data
+    experts = p.buffer.as_strided((T, top_k), (top_k, 1), at + n).data
     if T:
         address = p._at[0] + 4 * at
         _call("nvfp4_moe_route", logits, logits.data_ptr(), _KINDS[logits.dtype], ld, None if mask is None else mask.data_ptr(),
