@@ -110,6 +110,8 @@ struct Vec {
     }
 };
 
+// Whether the addresses are those of 32-bit words (NULL is).
+template <typename... P> bool words(const P*... p) { return ((0 | ... | (uintptr_t)p) & 3) == 0; }
 inline int elem_bytes(int kind) { return kind == NVFP4_F32 ? 4 : 2; }
 inline bool kind_ok(int kind) { return kind == NVFP4_F32 || kind == NVFP4_F16 || kind == NVFP4_BF16; }
 

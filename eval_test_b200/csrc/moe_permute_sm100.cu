@@ -371,11 +371,11 @@ extern "C" int nvfp4_moe_dispatch(const void* x, int kind, long long ld, const v
     if (rc) return rc;
     if (E <= 0) return NVFP4_ERR_SHAPE;
     const int size = elem_bytes(kind);
-    int dev = 0;
-    if ((rc = current_device(&dev))) return rc;
     const long long row_bytes = (long long)H * size;
     const int vec = common_alignment(16, {(uintptr_t)x, (uintptr_t)xs, (unsigned long long)(ld * size), (unsigned long long)row_bytes});
-    if (vec < size) return NVFP4_ERR_ALIGN;
+    if (vec < size || !words(rows, offsets)) return NVFP4_ERR_ALIGN;
+    int dev = 0;
+    if ((rc = current_device(&dev))) return rc;
     const PermuteArgs p{(const int*)rows, (const int*)offsets + E, T, k, H};
     const int row_vecs = (int)(row_bytes / vec);
     cudaStream_t st = (cudaStream_t)stream;
@@ -405,9 +405,9 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
     if (!kind_ok(kind) || !kind_ok(out_kind)) return NVFP4_ERR_UNSUPPORTED;
     int rc = check_sizes(T, k, H, ld);
     if (rc) return rc;
+    if ((uintptr_t)y % elem_bytes(kind) || (uintptr_t)out % elem_bytes(out_kind) || !words(weights, rows)) return NVFP4_ERR_ALIGN;
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;
-    if ((uintptr_t)y % elem_bytes(kind) || (uintptr_t)out % elem_bytes(out_kind) || (uintptr_t)weights % 4) return NVFP4_ERR_ALIGN;
     if (ld * elem_bytes(kind) >= (1ll << 32)) return NVFP4_ERR_UNSUPPORTED;      // (the kernel's row pitch is 32-bit bytes)
     const PermuteArgs p{(const int*)rows, nullptr, T, k, H};
     cudaStream_t st = (cudaStream_t)stream;
@@ -457,11 +457,11 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
     int rc = check_sizes(T, k, H, ld);
     if (rc) return rc;
     if (E <= 0 || ldo < 0) return NVFP4_ERR_SHAPE;
+    if ((uintptr_t)y % elem_bytes(kind) || (uintptr_t)dy % elem_bytes(kind) || (uintptr_t)dout % elem_bytes(out_kind) ||
+        !words(weights, rows, offsets, dweights))
+        return NVFP4_ERR_ALIGN;
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;
-    if ((uintptr_t)y % elem_bytes(kind) || (uintptr_t)dy % elem_bytes(kind) || (uintptr_t)dout % elem_bytes(out_kind) ||
-        (uintptr_t)weights % 4 || (uintptr_t)dweights % 4)
-        return NVFP4_ERR_ALIGN;
     if (ld * elem_bytes(kind) >= (1ll << 32) || (long long)H * elem_bytes(kind) >= (1ll << 32)) return NVFP4_ERR_UNSUPPORTED;
     const PermuteArgs p{(const int*)rows, (const int*)offsets + E, T, k, H};
     cudaStream_t st = (cudaStream_t)stream;
@@ -524,7 +524,7 @@ extern "C" int nvfp4_moe_dispatch_nvfp4(const void* x, int kind, long long ld, c
     const bool table = nvfp4_moe_dispatch_scratch(T, k, K) > 0;
     if (table && !scratch) return NVFP4_ERR_NULL;
     if (((uintptr_t)x & 15) || ld * elem_bytes(kind) % 16 || ((uintptr_t)packed & 15) || ((uintptr_t)sf_sw & 15) ||
-        (table && ((uintptr_t)scratch & 15)))
+        (table && ((uintptr_t)scratch & 15)) || !words(offsets, tiles, rows, slots, source))
         return NVFP4_ERR_ALIGN;
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;

@@ -573,6 +573,7 @@ extern "C" int nvfp4_moe_plan(const void* experts, int T, int E, int k, void* of
     if (T <= 0 || E <= 0 || k <= 0) return NVFP4_ERR_SHAPE;
     if (E > MOE_MAX_EXPERTS || k > MOE_MAX_CHOICES || (long long)T * k > MOE_MOST) return NVFP4_ERR_UNSUPPORTED;
     if (nvfp4_moe_plan_scratch(T, E, k) && !scratch) return NVFP4_ERR_NULL;
+    if (!words(experts, offsets, tiles, wide_tiles, rows, slots, source, scratch)) return NVFP4_ERR_ALIGN;
     const PlanArgs p{(const int*)experts, (int*)offsets, (int*)tiles, (int*)wide_tiles, (int*)rows, (int*)slots, (int*)source, (uint32_t*)scratch, T, E, k};
     return plan_choices(p, (cudaStream_t)stream);
 }
@@ -583,6 +584,8 @@ extern "C" int nvfp4_moe_route(const void* logits, int kind, long long ld, const
     if (!logits || !weights || !experts || !offsets || !tiles || !wide_tiles || !rows || !slots || !source) return NVFP4_ERR_NULL;
     int rc = check_route(kind, ld, T, E, k);
     if (rc) return rc;
+    if ((uintptr_t)logits % elem_bytes(kind) || !words(weights, experts, offsets, tiles, wide_tiles, rows, slots, source, scratch))
+        return NVFP4_ERR_ALIGN;
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;
@@ -599,6 +602,7 @@ extern "C" int nvfp4_moe_route_backward(const void* dweights, const void* logits
     if ((uintptr_t)dlogits & 15) return NVFP4_ERR_ALIGN;
     int rc = check_route(kind, ld, T, E, k);
     if (rc) return rc;
+    if ((uintptr_t)logits % elem_bytes(kind) || !words(dweights, weights, experts)) return NVFP4_ERR_ALIGN;
     int dev = 0;
     cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return (int)err;

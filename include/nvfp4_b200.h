@@ -139,7 +139,8 @@ int nvfp4_quantize_bf16(const void* x, void* packed, void* sf_sw, int rows, int 
  * are sorted stably by expert into R = T*k rows.  The group sizes stay on the device, so a whole layer can be captured
  * into a graph (eval/nvfp4_grouped_gemm/reference.py:137-201 takes them as a host list).  An expert id outside [0, E)
  * means "not routed": the copy has no row.  At most 2^31 - 2^20 copies, and as many elements in a row
- * (NVFP4_ERR_UNSUPPORTED).  No entry point keeps a workspace: what it needs is an argument.  The kernels are launched
+ * (NVFP4_ERR_UNSUPPORTED).  Tables, weights and elements lie on multiples of their size (NVFP4_ERR_ALIGN).  No entry
+ * point keeps a workspace: what it needs is an argument.  The kernels are launched
  * with programmatic dependent launch and wait for the kernel before them in the stream before they touch memory.
  * Element types of activations: */
 enum { NVFP4_F32 = 0, NVFP4_F16 = 1, NVFP4_BF16 = 2 };
