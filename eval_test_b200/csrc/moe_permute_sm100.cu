@@ -104,11 +104,13 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const uint8_t* x, long lo
     zero_tail(out, row_vecs, p);
 }
 
-// KU rows' loads of U vectors each are in flight at a time.  `pitch`: bytes between rows of y.  (Loads past L1 are faster
+// KU rows' loads of U vectors each are in flight at a time.  `pitch`: bytes between rows of y, in 64 bits only where it
+// has more than 32 (with 64 throughout the gradient keeps two pointers per row in registers: 8192 x 8 x 4002 fp16 297 us
+// against 221).  (Loads past L1 are faster
 // for few rows, 4096 x 2 x 2048 fp32 14.7 against 19.3 us, 8192 x 4 x 4096 bf16 54.6 / 56.3, and slower for eight, whose
 // loads the compiler then cannot place among the sums: 16384 x 8 x 4096 197 / 180.)
-template <typename TI, typename TO, int VN, int KU, int U, bool WEIGHTED>
-__global__ void __launch_bounds__(256, U >= 2 && VN > 1 ? 3 : 4) combine_kernel(const TI* y, unsigned pitch, const float* weights, TO* out,
+template <typename TI, typename TO, int VN, int KU, int U, bool WEIGHTED, typename PITCH>
+__global__ void __launch_bounds__(256, U >= 2 && VN > 1 ? 3 : 4) combine_kernel(const TI* y, PITCH pitch, const float* weights, TO* out,
                                                                       int row_vecs, const PermuteArgs p) {
     pdl_wait();
     pdl_launch();
@@ -147,8 +149,8 @@ __global__ void __launch_bounds__(256, U >= 2 && VN > 1 ? 3 : 4) combine_kernel(
 // GROUP threads per token (a warp, or a block for long rows): a vector of dout[t] is read once for KU of the token's
 // rows; their dot products stay in registers and are summed over the group at the end, in an order that depends on the
 // sizes alone.  `pitch`: bytes between rows of y.
-template <typename TI, typename TO, int VN, int GROUP, int KU, int U>
-__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* dout, long long ldo, const TI* y, unsigned pitch,
+template <typename TI, typename TO, int VN, int GROUP, int KU, int U, typename PITCH>
+__global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* dout, long long ldo, const TI* y, PITCH pitch,
                                                                   const float* weights, TI* dy, float* dw, int row_vecs,
                                                                   const PermuteArgs p) {
     __shared__ float part[8][KU];
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(256, 3) combine_backward_kernel(const TO* dout
     constexpr int PER_BLOCK = 256 / GROUP;
     pdl_wait();
     pdl_launch();
-    const unsigned out_pitch = (unsigned)p.H * (unsigned)sizeof(TI);
+    const PITCH out_pitch = (PITCH)p.H * (PITCH)sizeof(TI);
     for (long long t = (long long)blockIdx.x * PER_BLOCK + threadIdx.x / GROUP; t < p.T; t += (long long)gridDim.x * PER_BLOCK) {
         const TO* d = dout + t * ldo;
         for (int j0 = 0; j0 < p.k; j0 += KU) {
@@ -408,7 +410,7 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
     if ((uintptr_t)y % elem_bytes(kind) || (uintptr_t)out % elem_bytes(out_kind) || !words(weights, rows)) return NVFP4_ERR_ALIGN;
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;
-    if (ld * elem_bytes(kind) >= (1ll << 32)) return NVFP4_ERR_UNSUPPORTED;      // (the kernel's row pitch is 32-bit bytes)
+    const bool far = ld * elem_bytes(kind) >= (1ll << 32);       // rows that only a pitch of 64 bits reaches
     const PermuteArgs p{(const int*)rows, nullptr, T, k, H};
     cudaStream_t st = (cudaStream_t)stream;
     return by_type(kind, [&](auto ti) {
@@ -419,16 +421,16 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
             constexpr int VN = 16 / sizeof(TI);
             constexpr unsigned long long O = VN * sizeof(TO) < 16 ? VN * sizeof(TO) : 16;
             const bool wide = H % VN == 0 && ld % VN == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)out % O == 0;
-            const bool pair = sizeof(TI) == 2 && !wide && H % 2 == 0 && ld % 2 == 0 && (uintptr_t)y % 4 == 0 && (uintptr_t)out % (2 * sizeof(TO)) == 0;
+            const bool pair = sizeof(TI) == 2 && !wide && !far && H % 2 == 0 && ld % 2 == 0 && (uintptr_t)y % 4 == 0 && (uintptr_t)out % (2 * sizeof(TO)) == 0;
             const int row_vecs = wide ? H / VN : pair ? H / 2 : H;
-            auto go = [&](auto vn, auto ku, auto u) {
+            auto go = [&](auto vn, auto ku, auto u, auto pitch) {
+                using P = decltype(pitch);
                 constexpr int N = decltype(vn)::value, KU = decltype(ku)::value, U = decltype(u)::value;
                 const long long warps = (long long)T * ((row_vecs + 32 * U - 1) / (32 * U));
                 if (warps >= (1ll << 31)) return (int)NVFP4_ERR_UNSUPPORTED;
                 const int grid = grid_for(32 * warps, dev);
-                const unsigned pitch = (unsigned)(ld * sizeof(TI));
-                return launch_dependent(weights ? combine_kernel<TI, TO, N, KU, U, true> : combine_kernel<TI, TO, N, KU, U, false>, grid,
-                                        256, 0, 0, st, (const TI*)y, pitch, (const float*)weights, (TO*)out, row_vecs, p);
+                return launch_dependent(weights ? combine_kernel<TI, TO, N, KU, U, true, P> : combine_kernel<TI, TO, N, KU, U, false, P>,
+                                        grid, 256, 0, 0, st, (const TI*)y, pitch, (const float*)weights, (TO*)out, row_vecs, p);
             };
             using std::integral_constant;
             auto go_width = [&](auto vn) {
@@ -437,9 +439,15 @@ extern "C" int nvfp4_moe_combine(const void* y, int kind, long long ld, const vo
                 // 19.0 with two), and more where a vector is one or two elements (8192 x 8 x 4002 fp16, one, two, four
                 // vectors of eight rows: 192, 159, 297 us; 4001 wide 332, 275, 314)
                 constexpr int N = decltype(vn)::value;
-                if (k <= 2) return go(vn, integral_constant<int, 2>(), integral_constant<int, N == 8 ? 2 : 4>());
-                if (k <= 4) return go(vn, integral_constant<int, 4>(), integral_constant<int, 2>());
-                return go(vn, integral_constant<int, 8>(), integral_constant<int, N <= 2 ? 2 : 1>());
+                const unsigned pitch = (unsigned)(ld * sizeof(TI));
+                const auto two = integral_constant<int, 2>();
+                const auto of_two = integral_constant<int, N == 8 ? 2 : 4>();
+                if constexpr (N != 2) {
+                    if (far) return go(vn, two, of_two, (unsigned long long)ld * sizeof(TI));
+                }
+                if (k <= 2) return go(vn, two, of_two, pitch);
+                if (k <= 4) return go(vn, integral_constant<int, 4>(), two, pitch);
+                return go(vn, integral_constant<int, 8>(), integral_constant<int, N <= 2 ? 2 : 1>(), pitch);
             };
             if constexpr (sizeof(TI) == 2) {
                 if (pair) return go_width(integral_constant<int, 2>());
@@ -462,7 +470,7 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
         return NVFP4_ERR_ALIGN;
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;
-    if (ld * elem_bytes(kind) >= (1ll << 32) || (long long)H * elem_bytes(kind) >= (1ll << 32)) return NVFP4_ERR_UNSUPPORTED;
+    const bool far = ld * elem_bytes(kind) >= (1ll << 32) || (long long)H * elem_bytes(kind) >= (1ll << 32);
     const PermuteArgs p{(const int*)rows, (const int*)offsets + E, T, k, H};
     cudaStream_t st = (cudaStream_t)stream;
     return by_type(kind, [&](auto ti) {
@@ -473,26 +481,33 @@ extern "C" int nvfp4_moe_combine_backward(const void* dout, int out_kind, long l
             constexpr unsigned long long O = VN * sizeof(TO) < 16 ? VN * sizeof(TO) : 16;
             const bool wide = H % VN == 0 && ld % VN == 0 && ldo % VN == 0 && (uintptr_t)y % 16 == 0 && (uintptr_t)dy % 16 == 0 &&
                               (uintptr_t)dout % O == 0;
-            const bool pair = sizeof(TI) == 2 && !wide && H % 2 == 0 && ld % 2 == 0 && ldo % 2 == 0 && (uintptr_t)y % 4 == 0 &&
+            const bool pair = sizeof(TI) == 2 && !wide && !far && H % 2 == 0 && ld % 2 == 0 && ldo % 2 == 0 && (uintptr_t)y % 4 == 0 &&
                               (uintptr_t)dy % 4 == 0 && (uintptr_t)dout % (2 * sizeof(TO)) == 0;
             const int row_vecs = wide ? H / VN : pair ? H / 2 : H;
             // a warp per token where its lanes take at most four vectors each, and for few choices where there are tokens
             // enough for that (bf16, 4096 wide, a warp against a block: 16384 x 1 65 against 86 us, 8192 x 4 98 / 105; with
             // eight rows in registers a warp's loads no longer cover its stores: 16384 x 8 372 / 351)
-            const bool warp = row_vecs <= 128 || (k <= 4 && T >= 16 * sm_count(dev));
+            const bool warp = !far && (row_vecs <= 128 || (k <= 4 && T >= 16 * sm_count(dev)));
             const int grid = grid_for((long long)T * (warp ? 32 : 256), dev);
-            auto go = [&](auto vn, auto group, auto ku, auto u) {
+            auto go = [&](auto vn, auto group, auto ku, auto u, auto pitch) {
                 return launch_dependent(
-                    combine_backward_kernel<TI, TO, decltype(vn)::value, decltype(group)::value, decltype(ku)::value, decltype(u)::value>,
-                    grid, 256, 0, 0, st, (const TO*)dout, ldo, (const TI*)y, (unsigned)(ld * sizeof(TI)), (const float*)weights, (TI*)dy,
-                    (float*)dweights, row_vecs, p);
+                    combine_backward_kernel<TI, TO, decltype(vn)::value, decltype(group)::value, decltype(ku)::value, decltype(u)::value,
+                                            decltype(pitch)>,
+                    grid, 256, 0, 0, st, (const TO*)dout, ldo, (const TI*)y, pitch, (const float*)weights, (TI*)dy, (float*)dweights,
+                    row_vecs, p);
             };
             using std::integral_constant;
             auto go_group = [&](auto vn, auto group) {
                 constexpr int N = decltype(vn)::value;
-                if (k <= 2) return go(vn, group, integral_constant<int, 2>(), integral_constant<int, N <= 2 ? 8 : 2>());
-                if (k <= 4) return go(vn, group, integral_constant<int, 4>(), integral_constant<int, N <= 2 ? 4 : 2>());
-                return go(vn, group, integral_constant<int, 8>(), integral_constant<int, N <= 2 ? 2 : 1>());
+                const unsigned pitch = (unsigned)(ld * sizeof(TI));
+                const auto two = integral_constant<int, 2>();
+                const auto of_two = integral_constant<int, N <= 2 ? 8 : 2>();
+                if constexpr (N != 2 && decltype(group)::value > 32) {
+                    if (far) return go(vn, group, two, of_two, (unsigned long long)ld * sizeof(TI));
+                }
+                if (k <= 2) return go(vn, group, two, of_two, pitch);
+                if (k <= 4) return go(vn, group, integral_constant<int, 4>(), integral_constant<int, N <= 2 ? 4 : 2>(), pitch);
+                return go(vn, group, integral_constant<int, 8>(), integral_constant<int, N <= 2 ? 2 : 1>(), pitch);
             };
             auto go_width = [&](auto vn) {
                 return warp ? go_group(vn, integral_constant<int, 32>()) : go_group(vn, integral_constant<int, 256>());
