@@ -32,8 +32,11 @@
 //     to fp16, are turned over in a piece of shared memory that belongs to the warp, 16 tokens x 32 weight rows at a time,
 //     and a lane stores 16 of a token's outputs (32 bytes), or quantises them (they are one block).
 // Every mbarrier wait is bounded; on expiry the role records a status code and leaves its loop, the CTA still frees its
-// tensor memory and exits.  The epilogue's named barrier is reached by all of its warps or by none; the two hardware cluster
-// barriers (after set-up, before exit) are reached by every thread on every path.
+// tensor memory and exits.  Before that the issuer waits, again with a limit, for the products that it has issued and, where
+// it left its loop, for the stages that are still being filled: the epilogue may have given up in front of it, and what they
+// read and write belongs to the next CTA afterwards.  The epilogue's named barrier is reached by all of its warps or by none,
+// and by all lanes of a warp; the two hardware cluster barriers (after set-up, before exit) are reached by every thread on
+// every path.
 #include <cuda.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -209,7 +212,7 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
 
     extern __shared__ uint8_t smem_raw[];
     // same layout in both CTAs (remote arrivals and pair-wide commits address barriers by offset)
-    __shared__ __align__(8) uint64_t bars[2 * STAGES + 5];
+    __shared__ __align__(8) uint64_t bars[2 * STAGES + 6];
     __shared__ uint32_t tmem_base_slot;
     __shared__ int gave_up;
 
@@ -220,6 +223,7 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     const uint32_t acc_full0 = smem_u32(&bars[2 * STAGES]);     // [2] accumulator complete, signalled in both CTAs
     const uint32_t acc_empty0 = acc_full0 + 16;                 // [2] accumulator drained, leader's copy used
     const uint32_t ovl_free = acc_full0 + 32;                   // shared columns drained, leader's copy used
+    const uint32_t issued_done = acc_full0 + 40;                // every product of the launch is complete, leader's copy used
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) {
@@ -231,6 +235,7 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             mbar_init(acc_empty0 + 8 * b, 2 * x_epilogue_warps(NT));
         }
         mbar_init(ovl_free, 2 * x_epilogue_warps(NT));
+        mbar_init(issued_done, 1);
         gave_up = 0;
         fence_mbar_init();
         prefetch_tmap(&maps.a[0]);
@@ -368,6 +373,11 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
                     if (alive) tc_commit_pair(acc_full0 + 8 * buf, 3);      // accumulators complete in both CTAs
                 }
             }
+            tc_commit_pair(issued_done, 1);
+            if (!mbar_wait_cluster(issued_done, 0, p.budget_ns)) report_status(p.status, DEV_TIMEOUT_MMA_ACC);
+            // the stages that nothing was issued for, in their order; behind the last one that was filled, one budget
+            for (int s = 0; !alive && s < STAGES && mbar_wait_cluster(full0 + 8 * slot, phase, p.budget_ns); s++)
+                if (++slot == STAGES) { slot = 0; phase ^= 1; }
         }
     } else if (warp >= X_FIRST_EPILOGUE) {
         // ------------------------------------------------------------------ epilogue warps (both CTAs)
@@ -399,8 +409,10 @@ expert_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
                 if (!alive) break;
                 // one warp waits for the accumulator and the others for that warp (sixteen waiting warps took power from the
                 // rest of the board: 1 %).  If it gives up it says in which pass, so that all of them leave at the same barrier
-                if (warp == X_FIRST_EPILOGUE && !mbar_wait(acc_full0 + 8 * buf, (seq >> 1) & 1, p.budget_ns)) {
-                    if (lane == 0) {
+                // (the lanes wait each for itself, and the limit of one may pass just before another sees the accumulator)
+                if (warp == X_FIRST_EPILOGUE) {
+                    const bool there = __all_sync(0xffffffffu, mbar_wait(acc_full0 + 8 * buf, (seq >> 1) & 1, p.budget_ns));
+                    if (!there && lane == 0) {
                         report_status(p.status, DEV_TIMEOUT_EPILOGUE);
                         *(volatile int*)&gave_up = (int)seq + 1;
                     }
