@@ -34,7 +34,7 @@ _KINDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 class Plan:
     """How the copies of a batch are sorted (``nvfp4_moe_plan``).  One int32 buffer on the batch's device holds its six
     tables; the views are made when they are asked for (a call of the layer needs only their addresses)."""
-    __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "num_copies", "most_tiles", "_at")
+    __slots__ = ("buffer", "num_tokens", "top_k", "num_experts", "num_copies", "most_tiles", "_at", "_more")
 
     def __init__(self, num_tokens: int, top_k: int, num_experts: int, device: torch.device, more: int = 0):
         n, e = num_tokens * top_k, num_experts + 1
@@ -42,7 +42,8 @@ class Plan:
             raise ValueError(f"expected at most {MAX_COPIES} choices in a batch, got {n}")
         # behind the tables: the copies per expert of each block of a large sort, then `more` words for the caller
         scratch = _lib.load().nvfp4_moe_plan_scratch(num_tokens, num_experts, top_k) // 4 if n > 4096 else 0
-        size = 3 * e + 3 * n + scratch + more
+        self._more = 3 * e + 3 * n + scratch    # where the caller's words start
+        size = self._more + more
         # (no copies: nothing is launched, and every expert starts at row 0)
         self.buffer = torch.empty(size, dtype=torch.int32, device=device) if n else torch.zeros(size, dtype=torch.int32, device=device)
         self.num_tokens, self.top_k, self.num_experts, self.num_copies = num_tokens, top_k, num_experts, n
@@ -101,8 +102,8 @@ class Routing(NamedTuple):
     plan: Plan
 
 
-def _matrix(t: torch.Tensor, name: str, rows: int | None = None, cols: int | None = None) -> int:
-    """Checks ``[rows, cols]`` of a floating type whose rows are contiguous; returns the pitch in elements."""
+def _matrix(t: torch.Tensor, name: str, rows: int | None = None, cols: int | None = None):
+    """Checks ``[rows, cols]`` of a floating type whose rows are contiguous -> (rows, columns, pitch in elements)."""
     if not (isinstance(t, torch.Tensor) and t.is_cuda and t.dim() == 2 and t.dtype in _KINDS):
         raise ValueError(f"{name}: expected a CUDA float32 / float16 / bfloat16 matrix")
     have_rows, have_cols = t.shape
@@ -113,7 +114,7 @@ def _matrix(t: torch.Tensor, name: str, rows: int | None = None, cols: int | Non
     pitch, step = t.stride()
     if step != 1 and have_cols > 1:
         raise ValueError(f"{name}: the rows have to be contiguous, got strides {t.stride()}")
-    return pitch if have_rows > 1 else have_cols
+    return have_rows, have_cols, pitch if have_rows > 1 else have_cols
 
 
 def _choices(t: torch.Tensor, name: str, dtype: torch.dtype, shape=None) -> None:
@@ -194,8 +195,7 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torc
     NaN and -inf entries, and the rows of tokens whose ``mask`` [T] (bool) is false, are never chosen and take no part in
     the sum; where fewer than ``top_k`` candidates are left the expert is -1 and the weight 0.  Several +inf entries share
     the whole weight."""
-    ld = _matrix(logits, "logits")
-    T, E = logits.shape
+    T, E, ld = _matrix(logits, "logits")
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"logits: expected 1 to {MAX_EXPERTS} experts, got {E}")
     if not 1 <= top_k <= min(E, MAX_CHOICES):
@@ -209,7 +209,7 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torc
     # tensors of their own for autograd, so that weights changed in place do not pass for changed choices or tables
     n = T * top_k
     p = Plan(T, top_k, E, device, 2 * n)
-    at = p.buffer.shape[0] - 2 * n
+    at = p._more
     weights = p.buffer.view(torch.float32).as_strided((T, top_k), (top_k, 1), at).data
     experts = p.buffer.as_strided((T, top_k), (top_k, 1), at + n).data
     if T:
@@ -223,8 +223,7 @@ def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, weights: to
                    renormalize: bool = True) -> torch.Tensor:
     """Gradient of ``route``'s weights with respect to ``logits`` (same type and shape; contiguous), from what ``route``
     took and returned.  Entries that took no part have gradient 0."""
-    ld = _matrix(logits, "logits")
-    T, E = logits.shape
+    T, E, ld = _matrix(logits, "logits")
     _choices(experts, "experts", torch.int32)
     k = experts.shape[1]
     if not 1 <= E <= MAX_EXPERTS or not 1 <= k <= min(E, MAX_CHOICES):
@@ -243,8 +242,7 @@ def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, weights: to
 def dispatch(x: torch.Tensor, plan: Plan) -> torch.Tensor:
     """``x`` [T, H] -> [T * k, H] of the same type: every token's row at the rows of its copies."""
     T, k = plan.num_tokens, plan.top_k
-    ld = _matrix(x, "x", T)
-    H = x.shape[1]
+    _, H, ld = _matrix(x, "x", T)
     _same_device(x, plan.buffer)
     out = x.new_empty((T * k, H))
     if out.numel():
@@ -262,8 +260,7 @@ def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dt
     """``y`` [T * k, H], rows sorted by expert -> [T, H]: the sum of each token's rows times ``weights`` [T, k] (float32; none:
     the plain sum), in fp32, rounded once to ``dtype`` (default: that of ``y``).  Choices that are not routed add nothing."""
     T, k = plan.num_tokens, plan.top_k
-    ld = _matrix(y, "y", T * k)
-    H = y.shape[1]
+    _, H, ld = _matrix(y, "y", T * k)
     dtype = y.dtype if dtype is None else dtype
     if dtype not in _KINDS:
         raise ValueError(f"dtype: expected float32, float16 or bfloat16, got {dtype}")
@@ -281,8 +278,8 @@ def combine_backward(grad_out: torch.Tensor, y: torch.Tensor, plan: Plan, weight
     """Gradients of ``combine`` with weights: ``grad_out`` [T, H] -> (that of ``y``, same type, rows that belong to no copy 0;
     that of ``weights`` [T, k], 0 where a choice is not routed)."""
     T, k = plan.num_tokens, plan.top_k
-    ldo, ld = _matrix(grad_out, "grad_out", T), _matrix(y, "y", T * k, grad_out.shape[1])
-    H = y.shape[1]
+    _, H, ldo = _matrix(grad_out, "grad_out", T)
+    ld = _matrix(y, "y", T * k, H)[2]
     _choices(weights, "weights", torch.float32, (T, k))
     _same_device(y, grad_out, plan.buffer, weights)
     dy = y.new_empty((T * k, H))
@@ -299,8 +296,7 @@ def dispatch_nvfp4(x: torch.Tensor, plan: Plan):
     ``[T * k, K/2, 1]`` float4_e2m1fn_x2, 6-D swizzled scales of the experts' 128-row tiles, ``plan.most_tiles`` of them).
     Scale bytes of rows that do not exist have no meaning.  K is a multiple of 64."""
     T, k = plan.num_tokens, plan.top_k
-    ld = _matrix(x, "x", T)
-    K = x.shape[1]
+    _, K, ld = _matrix(x, "x", T)
     if K % 64 or not K:
         raise ValueError(f"x: the width has to be a multiple of 64, got {K}")
     _same_device(x, plan.buffer)
