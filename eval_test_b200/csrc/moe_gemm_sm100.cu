@@ -561,7 +561,8 @@ int expert_product(const void* a, const void* sfa_sw, const void* b, const void*
                          R, E, N, K, alpha, status_word_anywhere(dev), wait_budget_ns()};
     cudaStream_t st = (cudaStream_t)stream;
     // few rows per expert on average (64 experts, K = 7168, experts liked unequally, NT = 128 against 256): 32 rows 161
-    // against 169 us, 64: 172 / 175, 96: 188 / 187, 128: 217 / 204; DUAL 32: 159 / 172, 96: 182 / 200, 128: 213 / 208
+    // against 169 us, 64: 172 / 175, 96: 188 / 187, 128: 217 / 204; DUAL 32: 159 / 172, 96: 182 / 200, 128: 213 / 208.  The
+    // host knows the number of copies only, so choices that are not routed count as rows here
     const bool few = R <= 96ll * E;
     return few ? launch_experts<DUAL, QOUT, 128>(maps, p, dev, st) : launch_experts<DUAL, QOUT, 256>(maps, p, dev, st);
 }

@@ -16,7 +16,9 @@ behind the last routed copy are zero in every sorted buffer made here.
 
 Expert weights are one batched operand, as ``quantize.quantize_operand`` makes it of ``[E, N, K]``: packed codes
 ``[N, K/2, E]`` and the 6-D swizzled view of their scales.  The gradients of the 16- and 32-bit operations are functions
-of their own (``*_backward``); there are none of the NVFP4 products.
+of their own (``*_backward``); there are none of the NVFP4 products.  Nothing here registers with autograd: results never
+require gradients, whatever their inputs do, so a training step calls these functions from ``torch.autograd.Function``s
+of its own.
 """
 from __future__ import annotations
 
@@ -24,7 +26,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import _args, _lib, formats as F
+from . import _args, _lib
 
 MAX_EXPERTS, MAX_CHOICES = 1024, 32
 MAX_COPIES = (1 << 31) - (1 << 20)      # also of a matrix: rows, columns
@@ -194,7 +196,7 @@ def route(logits: torch.Tensor, top_k: int, renormalize: bool = True, mask: torc
 
     NaN and -inf entries, and the rows of tokens whose ``mask`` [T] (bool) is false, are never chosen and take no part in
     the sum; where fewer than ``top_k`` candidates are left the expert is -1 and the weight 0.  Several +inf entries share
-    the whole weight."""
+    the whole weight.  The weights do not require gradients: theirs is ``route_backward``."""
     T, E, ld = _matrix(logits, "logits")
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"logits: expected 1 to {MAX_EXPERTS} experts, got {E}")
@@ -240,7 +242,8 @@ def route_backward(grad_weights: torch.Tensor, logits: torch.Tensor, weights: to
 
 
 def dispatch(x: torch.Tensor, plan: Plan) -> torch.Tensor:
-    """``x`` [T, H] -> [T * k, H] of the same type: every token's row at the rows of its copies."""
+    """``x`` [T, H] -> [T * k, H] of the same type: every token's row at the rows of its copies.  The result does not
+    require gradients: its gradient is ``dispatch_backward``."""
     T, k = plan.num_tokens, plan.top_k
     _, H, ld = _matrix(x, "x", T)
     _same_device(x, plan.buffer)
@@ -258,7 +261,8 @@ def dispatch_backward(grad_rows: torch.Tensor, plan: Plan) -> torch.Tensor:
 
 def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dtype: torch.dtype | None = None) -> torch.Tensor:
     """``y`` [T * k, H], rows sorted by expert -> [T, H]: the sum of each token's rows times ``weights`` [T, k] (float32; none:
-    the plain sum), in fp32, rounded once to ``dtype`` (default: that of ``y``).  Choices that are not routed add nothing."""
+    the plain sum), in fp32, rounded once to ``dtype`` (default: that of ``y``).  Choices that are not routed add nothing.
+    The result does not require gradients: theirs are ``combine_backward``."""
     T, k = plan.num_tokens, plan.top_k
     _, H, ld = _matrix(y, "y", T * k)
     dtype = y.dtype if dtype is None else dtype
@@ -276,7 +280,8 @@ def combine(y: torch.Tensor, plan: Plan, weights: torch.Tensor | None = None, dt
 
 def combine_backward(grad_out: torch.Tensor, y: torch.Tensor, plan: Plan, weights: torch.Tensor):
     """Gradients of ``combine`` with weights: ``grad_out`` [T, H] -> (that of ``y``, same type, rows that belong to no copy 0;
-    that of ``weights`` [T, k], 0 where a choice is not routed)."""
+    that of ``weights`` [T, k], 0 where a choice is not routed).  The order of a dot product's sum follows from the sizes,
+    the types, the alignment of addresses and pitches and the number of SMs."""
     T, k = plan.num_tokens, plan.top_k
     _, H, ldo = _matrix(grad_out, "grad_out", T)
     ld = _matrix(y, "y", T * k, H)[2]
@@ -356,7 +361,8 @@ def expert_dual_gemm(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0) -> torch
 
 def expert_dual_gemm_nvfp4(a, sfa, b1, sfb1, b2, sfb2, plan: Plan, alpha=1.0):
     """``expert_dual_gemm`` with its rows quantised to NVFP4, bit for bit what quantising the fp16 rows gives -> (operand
-    ``[T * k, N/2, 1]``, 6-D scales): ``a`` and ``sfa`` of the next product of the same plan."""
+    ``[T * k, N/2, 1]``, 6-D scales): ``a`` and ``sfa`` of the next product of the same plan, for which N has to be a
+    multiple of 256 (it is that product's K)."""
     ptrs, alpha, R, E, N, K = _products(a, sfa, (b1, sfb1, b2, sfb2), plan, alpha)
     packed, scales = _new_operand(a, R, plan.most_tiles * 128, N)
     if R:

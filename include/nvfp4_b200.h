@@ -179,7 +179,8 @@ int nvfp4_moe_dispatch(const void* x, int kind, long long ld, const void* rows, 
 int nvfp4_moe_combine(const void* y, int kind, long long ld, const void* weights, const void* rows, int T, int k, int H,
                       void* out, int out_kind, void* stream);
 /* The gradient of nvfp4_moe_combine: dy [T*k][H] (`kind`; rows behind the last copy become 0) and dweights [T][k]
- * (fp32; 0 where a copy has no row) from dout [T][H] (out_kind, rows `ldo` elements apart). */
+ * (fp32; 0 where a copy has no row) from dout [T][H] (out_kind, rows `ldo` elements apart).  The order of a dot product's
+ * sum follows from sizes, types, alignment and the number of SMs. */
 int nvfp4_moe_combine_backward(const void* dout, int out_kind, long long ldo, const void* y, int kind, long long ld,
                                const void* weights, const void* rows, const void* offsets, int T, int E, int k, int H,
                                void* dy, void* dweights, void* stream);
@@ -205,7 +206,7 @@ int nvfp4_moe_gemm(const void* a, const void* sfa_sw, const void* b, const void*
 int nvfp4_moe_dual_gemm(const void* a, const void* sfa_sw, const void* b1, const void* sfb1_sw, const void* b2,
                         const void* sfb2_sw, const void* offsets, const void* tiles, const void* wide_tiles,
                         const void* alphas, void* c, int R, int E, int N, int K, float alpha, void* stream);
-/* The same with the result quantised, ready to be `a` of the next product of the same plan: c_packed [R][N/2], sfc_sw
+/* The same with the result quantised, ready to be `a` of the next product of the same plan (where N % 256 == 0): c_packed [R][N/2], sfc_sw
  * [tiles][N/64][512]; bit for bit nvfp4_quantize_f16 of the fp16 rows. */
 int nvfp4_moe_dual_gemm_nvfp4(const void* a, const void* sfa_sw, const void* b1, const void* sfb1_sw, const void* b2,
                               const void* sfb2_sw, const void* offsets, const void* tiles, const void* wide_tiles,
