@@ -38,3 +38,22 @@ def test_gradient_of_a_row_of_more_than_32_bits_of_bytes():
     assert float(dw) == 7.0                                         # (sums of small whole numbers are exact)
     assert torch.equal(dy, d.mul_(0.5))
     assert torch.equal(moe.combine(y, plan, torch.full((1, 1), 0.5, device="cuda")), y.mul_(0.5))
+
+
+# more choices than the two rows that are taken at a time, and the longest pitch that 32 bits hold
+@pytest.mark.parametrize("dtype,pitch,k", [(F32, (1 << 30) + 4, 5), (F16, (1 << 31) + 1, 5), (F32, (1 << 30) - 4, 3), (BF16, (1 << 31) - 1, 3)])
+def test_choices_of_one_token_far_apart(dtype, pitch, k):
+    from eval_test_b200 import moe
+    H = 600
+    plan = moe.plan(choices(1, 7, k, 0.3, seed=3), 7)
+    g = torch.Generator().manual_seed(4)
+    near = torch.randn((k, H), generator=g).to(dtype).cuda()
+    far = torch.empty((k - 1) * pitch + H, dtype=dtype, device="cuda").as_strided((k, H), (pitch, 1))
+    far.copy_(near)
+    w, d = torch.randn((1, k), generator=g).cuda(), torch.randn((1, H), generator=g).cuda()
+    assert torch.equal(moe.combine(far, plan, w, dtype=F32), moe.combine(near, plan, w, dtype=F32))
+    got, want = moe.combine_backward(d, far, plan, w), moe.combine_backward(d, near, plan, w)
+    assert torch.equal(got[0], want[0])
+    rows = plan.rows.long()
+    size = torch.where(rows >= 0, (d.double()[:, None, :] * near.double()[rows.clamp(min=0)]).abs().sum(2), 0.0)
+    assert torch.all((got[1].double() - want[1].double()).abs() <= 2 * H * EPS32 * size)
